@@ -395,6 +395,68 @@ int32_t tylo_b200_softmax_fwd(void* Y, const void* X, int64_t M, int64_t N, int3
 int32_t tylo_b200_softmax_bwd(void* dX, const void* dY, const void* Y, int64_t M, int64_t N,
                               int32_t dtype, tylo_stream_t stream);
 
+/* ---- scores and losses over a vocabulary ---------------------------------------------------------
+ * No counterpart in the reference, whose softmax (src/softmax/softmax.jl:96-136) stands at the same place: what a model's
+ * logits are turned into, without an array of probabilities in memory.
+ * X (M,N): N rows (tokens) of M logits each, contiguous along dim 1; rows start ldx >= M elements apart, so a row may be part of
+ * a wider (padded) buffer, of which nothing but the M logits is read or written.  Statistics, weights and results are fp32.  With
+ * y = (x - max x) / temperature, L = sum exp(y), p = exp(y) / L per row:
+ *  - Masked logits may be -Inf or the lowest value of the type.  A row of nothing but -Inf has no probability anywhere: its
+ *    statistics are (-Inf, 0), its log probabilities -Inf, its entropy 0, its gradient zero.  A NaN or +Inf makes its row NaN.
+ *  - Token ids are 0-based int32.  An id outside [0, M) stands for "no token" (padding).
+ *  - dX has the rows of X (same M, N, ldx) and may be the same memory as X.  A row whose weights are all zero gets zeros.
+ *  - Results do not depend on the order in which the GPU works: equal inputs give equal bits. */
+#define TYLO_TOP_MAX 256       /* most alternatives per row */
+#define TYLO_DISTILL_MAX 1024  /* most teacher entries per row */
+
+/* Logp (N,): y[targets[n]] - log L, 0 where there is no token; goes with targets (both or neither).
+ * Entropy (N,), nullable: -sum p log p.
+ * TopLogp, TopIndex (top,N), with top > 0: the `top` largest logits of each row in falling order, as log probabilities and
+ * indices; among equal logits the lowest index first, a NaN before everything.
+ * Mx, L (N,), nullable together: checkpoints for the backward, the row's largest logit and sum exp(y). */
+int32_t tylo_b200_token_logprobs_fwd(float* Logp, float* Entropy, float* TopLogp, int32_t* TopIndex,
+                                     float* Mx, float* L,
+                                     const void* X, const int32_t* targets, int32_t top,
+                                     int64_t M, int64_t N, int64_t ldx, float temperature, int32_t dtype,
+                                     tylo_stream_t stream);
+/* dX = dLogp ([j = target] - p) / temperature - dEntropy p (log p + Entropy) / temperature (overwrites dX).
+ * dLogp goes with targets; dEntropy is nullable and needs the forward's Entropy.  At least one of the two weights is given. */
+int32_t tylo_b200_token_logprobs_bwd(void* dX, const float* dLogp, const float* dEntropy,
+                                     const void* X, const int32_t* targets,
+                                     const float* Entropy, const float* Mx, const float* L,
+                                     int64_t M, int64_t N, int64_t ldx, float temperature, int32_t dtype,
+                                     tylo_stream_t stream);
+/* Both in one launch, for weights that are known before the forward (next-token training: dLogp = -1 / tokens).  Logp and
+ * Entropy are nullable. */
+int32_t tylo_b200_token_logprobs_fwd_bwd(float* Logp, float* Entropy, void* dX,
+                                         const float* dLogp, const float* dEntropy,
+                                         const void* X, const int32_t* targets,
+                                         int64_t M, int64_t N, int64_t ldx, float temperature, int32_t dtype,
+                                         tylo_stream_t stream);
+
+/* Distillation from a teacher's top logits: teacher (K,N) fp32 and index (K,N) hold K entries per row, in any order.
+ * renormalize != 0: the teacher's probabilities are P_k = softmax over the row's entries of teacher / teacher_temperature;
+ * renormalize == 0: P_k = exp(teacher / teacher_temperature) as it is (log probabilities of a teacher whose other tokens are left
+ * out).  Loss (N,) = sum_k P_k (log P_k - log p[index_k]).
+ * Entries with an id outside [0, M) are left out, of the normalisation too; a row without entries has loss 0 and gradient 0.  The
+ * same id may occur more than once: each entry counts.  The alternatives of tylo_b200_token_logprobs_fwd are valid entries
+ * (with its temperature already in them: teacher_temperature = 1). */
+int32_t tylo_b200_distill_fwd(float* Loss, float* Mx, float* L,
+                              const void* X, const float* teacher, const int32_t* index, int32_t K,
+                              int64_t M, int64_t N, int64_t ldx, float temperature, float teacher_temperature,
+                              int32_t renormalize, int32_t dtype, tylo_stream_t stream);
+/* dX_j = dLoss (p_j sum_k P_k - sum_{k: index_k = j} P_k) / temperature (overwrites dX); Mx, L from the forward. */
+int32_t tylo_b200_distill_bwd(void* dX, const float* dLoss,
+                              const void* X, const float* teacher, const int32_t* index,
+                              const float* Mx, const float* L, int32_t K,
+                              int64_t M, int64_t N, int64_t ldx, float temperature, float teacher_temperature,
+                              int32_t renormalize, int32_t dtype, tylo_stream_t stream);
+/* Both in one launch, for weights that are known before the forward. */
+int32_t tylo_b200_distill_fwd_bwd(float* Loss, void* dX, const float* dLoss,
+                                  const void* X, const float* teacher, const int32_t* index, int32_t K,
+                                  int64_t M, int64_t N, int64_t ldx, float temperature, float teacher_temperature,
+                                  int32_t renormalize, int32_t dtype, tylo_stream_t stream);
+
 /* ---- RMSNorm -----------------------------------------------------------------------------------
  * rms_norm! → rms_norm_fwd (src/norm/rms_norm.jl:115-128, kernel :6-32).
  * X, Y (M,N), W (M,), optional Rstd fp32 (N,):  y = x * rstd * (w + offset). */

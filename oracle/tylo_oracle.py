@@ -462,3 +462,77 @@ def layer_norm_bwd_ref(dY, X, W, *, eps):
     dW = np.sum(dY * xhat, axis=0)
     dB = np.sum(dY, axis=0)
     return dX, dW, dB, mean[..., 0], rstd[..., 0]
+
+
+# ---- scores and losses over a vocabulary (no counterpart in the reference) --------------------------------------
+def vocab_stats_ref(X, temperature=1.0):
+    """Per row of X (N, M): log p (N, M), p (N, M), entropy (N,).  A row of nothing but -Inf has no probability: log p = -Inf, p = 0,
+    entropy 0."""
+    X = np.asarray(X, dtype=np.float64)
+    mx = X.max(axis=1, keepdims=True)
+    with np.errstate(invalid="ignore", divide="ignore"):
+        y = np.where(np.isneginf(mx), -np.inf, (X - mx) / temperature)
+        total = np.exp(y).sum(axis=1, keepdims=True)
+        logp = y - np.where(total == 0, 0.0, np.log(total))
+    p = np.exp(logp)
+    entropy = -np.where(p > 0, p * np.where(p > 0, logp, 0.0), 0.0).sum(axis=1)
+    return logp, p, entropy
+
+
+def token_logprobs_ref(X, targets, temperature=1.0):
+    """(log probability of each row's target, entropy); 0 where the target is outside [0, M)."""
+    logp, _, entropy = vocab_stats_ref(X, temperature)
+    t = np.asarray(targets)
+    has = (t >= 0) & (t < logp.shape[1])
+    return np.where(has, logp[np.arange(len(t)), np.where(has, t, 0)], 0.0), entropy
+
+
+def top_alternatives_ref(X, top):
+    """Indices of the `top` largest entries per row, NaN before everything, the lowest index first among equals."""
+    X = np.asarray(X, dtype=np.float64)
+    return np.stack([np.lexsort((np.arange(X.shape[1]), -np.where(np.isnan(r), 0.0, r), ~np.isnan(r)))[:top] for r in X])
+
+
+def token_logprobs_bwd_ref(dlogp, d_entropy, X, targets, temperature=1.0):
+    logp, p, entropy = vocab_stats_ref(X, temperature)
+    N, M = p.shape
+    t = np.asarray(targets)
+    has = (t >= 0) & (t < M) & (p.sum(axis=1) > 0)
+    g = np.where(has, np.asarray(dlogp, dtype=np.float64), 0.0)
+    hot = np.zeros((N, M))
+    hot[np.arange(N)[has], t[has]] = 1.0
+    d = g[:, None] * (hot - p)
+    d -= np.asarray(d_entropy, dtype=np.float64)[:, None] * np.where(p > 0, p * (np.where(p > 0, logp, 0.0) + entropy[:, None]), 0.0)
+    return d / temperature
+
+
+def _teacher_ref(teacher, index, M, teacher_temperature, renormalize):
+    z = np.asarray(teacher, dtype=np.float64) / teacher_temperature
+    index = np.asarray(index)
+    z = np.where((index >= 0) & (index < M), z, -np.inf)
+    if renormalize:
+        mx = z.max(axis=1, keepdims=True)
+        mx = np.where(np.isneginf(mx), 0.0, mx)
+        total = np.exp(z - mx).sum(axis=1, keepdims=True)
+        z = z - mx - np.where(total == 0, 0.0, np.log(np.where(total == 0, 1.0, total)))
+    return z, np.exp(z)
+
+
+def distill_ref(X, teacher, index, temperature=1.0, teacher_temperature=1.0, renormalize=True):
+    logq, _, _ = vocab_stats_ref(X, temperature)
+    logp, p = _teacher_ref(teacher, index, logq.shape[1], teacher_temperature, renormalize)
+    at = np.clip(np.asarray(index), 0, logq.shape[1] - 1)
+    with np.errstate(invalid="ignore"):
+        return np.where(p > 0, p * (logp - np.take_along_axis(logq, at, axis=1)), 0.0).sum(axis=1)
+
+
+def distill_bwd_ref(dloss, X, teacher, index, temperature=1.0, teacher_temperature=1.0, renormalize=True):
+    _, q, _ = vocab_stats_ref(X, temperature)
+    N, M = q.shape
+    _, p = _teacher_ref(teacher, index, M, teacher_temperature, renormalize)
+    d = q * p.sum(axis=1, keepdims=True)
+    index = np.asarray(index)
+    for n in range(N):
+        live = (index[n] >= 0) & (index[n] < M)
+        np.subtract.at(d[n], index[n][live], p[n][live])
+    return np.where(q.sum(axis=1, keepdims=True) > 0, d, 0.0) * np.asarray(dloss, dtype=np.float64)[:, None] / temperature

@@ -103,6 +103,12 @@ _SIGS = {
     "tylo_b200_peer_close": [_ptr],
     "tylo_b200_softmax_fwd": [_ptr, _ptr, _i64, _i64, _i32, _ptr],
     "tylo_b200_softmax_bwd": [_ptr, _ptr, _ptr, _i64, _i64, _i32, _ptr],
+    "tylo_b200_token_logprobs_fwd": [_ptr] * 8 + [_i32] + [_i64] * 3 + [_f32, _i32, _ptr],
+    "tylo_b200_token_logprobs_bwd": [_ptr] * 8 + [_i64] * 3 + [_f32, _i32, _ptr],
+    "tylo_b200_token_logprobs_fwd_bwd": [_ptr] * 7 + [_i64] * 3 + [_f32, _i32, _ptr],
+    "tylo_b200_distill_fwd": [_ptr] * 6 + [_i32] + [_i64] * 3 + [_f32, _f32, _i32, _i32, _ptr],
+    "tylo_b200_distill_bwd": [_ptr] * 7 + [_i32] + [_i64] * 3 + [_f32, _f32, _i32, _i32, _ptr],
+    "tylo_b200_distill_fwd_bwd": [_ptr] * 6 + [_i32] + [_i64] * 3 + [_f32, _f32, _i32, _i32, _ptr],
     "tylo_b200_rms_norm_fwd": [_ptr] * 4 + [_i64, _i64, _f32, _f32, _i32, _ptr],
     "tylo_b200_rms_norm_bwd": [_ptr] * 7 + [_i32, _i64, _i64, _f32, _i32, _ptr],
     "tylo_b200_layer_norm_fwd": [_ptr] * 6 + [_i64, _i64, _f32, _i32, _ptr],
@@ -1118,6 +1124,251 @@ def grad_softmax(dY, Y):
     Xd = Duplicated(Y, torch.empty_like(Y))
     grad_softmax_(Duplicated(Y, dY), Xd)
     return Xd.shadow
+
+
+# ---------------------------------------------------------------------------------------------
+# scores and losses over a vocabulary (no counterpart in the reference; they stand beside its softmax)
+# ---------------------------------------------------------------------------------------------
+TOP_MAX, DISTILL_MAX = 256, 1024      # TYLO_TOP_MAX, TYLO_DISTILL_MAX
+
+
+class LogprobCheckpoints(NamedTuple):
+    M: torch.Tensor      # (N,) fp32: the row's largest logit
+    L: torch.Tensor      # (N,) fp32: sum exp((x - M) / temperature)
+
+
+class TopAlternatives(NamedTuple):
+    logp: torch.Tensor   # (N, K) fp32, falling
+    index: torch.Tensor  # (N, K) int32
+
+
+class TokenLogprobs(NamedTuple):
+    logp: Optional[torch.Tensor]
+    entropy: Optional[torch.Tensor]
+    top: Optional[TopAlternatives]
+
+
+def allocate_checkpoints_token_logprobs(X) -> LogprobCheckpoints:
+    """Also the checkpoints of ``distill_``."""
+    f = dict(dtype=torch.float32, device=X.device)
+    return LogprobCheckpoints(torch.empty(X.shape[0], **f), torch.empty(X.shape[0], **f))
+
+
+def allocate_top_alternatives(X, top: int) -> TopAlternatives:
+    N = X.shape[0]
+    return TopAlternatives(torch.empty(N, top, dtype=torch.float32, device=X.device),
+                           torch.empty(N, top, dtype=torch.int32, device=X.device))
+
+
+def _logits(X):
+    """(M, N, row stride) of a matrix of logits: rows are contiguous and may lie in a wider buffer."""
+    if X.dim() != 2:
+        raise ValueError("expected a matrix of logits (N, M)")
+    N, M = X.shape
+    sn, sm = X.stride()
+    if N == 1:
+        sn = max(sn, M)
+    if (sm != 1 and M != 1) or sn < M:
+        raise ValueError("rows of logits must be contiguous and must not overlap")
+    return M, N, sn
+
+
+def _row_array(name, t, shape, dtype, X):
+    if t is None:
+        return
+    if tuple(t.shape) != shape or t.dtype != dtype:
+        raise ValueError(f"{name}: expected {dtype} of shape {shape}, got {t.dtype} of shape {tuple(t.shape)}")
+    if t.device != X.device:
+        raise ValueError(f"{name} is on {t.device}, the logits on {X.device}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name}: arrays must be dense")
+
+
+def _logit_grad(X, dX, ld):
+    """The gradient has the rows of the logits: same shape, type, device and distance between rows."""
+    if dX.shape != X.shape or dX.dtype != X.dtype or dX.device != X.device or _logits(dX)[2] != ld and X.shape[0] != 1:
+        raise ValueError("the gradient must have the shape, type, device and row stride of the logits")
+
+
+class _on:
+    """Makes a tensor's device the current one for a call, so that streams and launches are that device's."""
+
+    __slots__ = ("index", "before")
+
+    def __init__(self, X):
+        self.index = X.device.index
+        if not X.is_cuda:
+            raise ValueError("libtylo_b200 takes device arrays (there is no CPU path)")
+
+    def __enter__(self):
+        self.before = torch.cuda.current_device()
+        if self.before != self.index:
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc):
+        if self.before != self.index:
+            torch.cuda.set_device(self.before)
+
+
+def _like_logits(X, ld):
+    """An uninitialised gradient of X with its row stride."""
+    N, M = X.shape
+    return torch.empty_strided((N, M), (ld, 1), dtype=X.dtype, device=X.device)
+
+
+def token_logprobs_(logp, X, targets, *, temperature=1.0, entropy=None, top: Optional[TopAlternatives] = None, checkpoints=None):
+    """Log probabilities of ``targets`` (N,) int32 under softmax(X / temperature), written to ``logp`` (N,) fp32.  Per row also,
+    where a buffer is given: ``entropy`` (N,) fp32, the largest alternatives ``top`` and the ``checkpoints`` of the backward.
+    ``logp`` and ``targets`` may both be None.  X (N, M): rows may lie in a wider buffer.  A target outside [0, M) is padding:
+    its log probability is 0.  Among equal logits the lowest index is the first alternative."""
+    pX, pl, pe = primal(X), primal(logp), primal(entropy)
+    M, N, ld = _logits(pX)
+    _row_array("logp", pl, (N,), torch.float32, pX)
+    _row_array("targets", targets, (N,), torch.int32, pX)
+    _row_array("entropy", pe, (N,), torch.float32, pX)
+    K = 0
+    tl = ti = cm = cl = None
+    if top is not None:
+        tl, ti = top
+        K = int(tl.shape[-1])
+        _row_array("top.logp", tl, (N, K), torch.float32, pX)
+        _row_array("top.index", ti, (N, K), torch.int32, pX)
+        if K == 0:
+            tl = ti = None
+    if checkpoints is not None:
+        cm, cl = checkpoints
+        _row_array("checkpoints.M", cm, (N,), torch.float32, pX)
+        _row_array("checkpoints.L", cl, (N,), torch.float32, pX)
+    with _on(pX):
+        _check(_lib.tylo_b200_token_logprobs_fwd(_p(pl), _p(pe), _p(tl), _p(ti), _p(cm), _p(cl), _p(pX), _p(targets), K, M, N, ld,
+                                                 float(temperature), _dtype(pX), _stream()))
+    return logp
+
+
+def token_logprobs(X, targets=None, *, temperature=1.0, entropy=False, top=0, checkpoints=None) -> TokenLogprobs:
+    N = X.shape[0]
+    f = dict(dtype=torch.float32, device=X.device)
+    out = TokenLogprobs(torch.empty(N, **f) if targets is not None else None, torch.empty(N, **f) if entropy else None,
+                        allocate_top_alternatives(X, top) if top else None)
+    token_logprobs_(out.logp, X, targets, temperature=temperature, entropy=out.entropy, top=out.top, checkpoints=checkpoints)
+    return out
+
+
+def _logprob_weights(logp, targets, entropy, pX, N):
+    """(dlogp, entropy, d_entropy) of a backward call, checked."""
+    dl = None if logp is None else logp.shadow
+    pe, de = (None, None) if entropy is None else (entropy.primal, entropy.shadow)
+    _row_array("logp's weights", dl, (N,), torch.float32, pX)
+    _row_array("targets", targets, (N,), torch.int32, pX)
+    _row_array("entropy", pe, (N,), torch.float32, pX)
+    _row_array("entropy's weights", de, (N,), torch.float32, pX)
+    return dl, pe, de
+
+
+def grad_token_logprobs_(logp: Optional[Duplicated], X: Duplicated, targets, *, checkpoints, entropy: Optional[Duplicated] = None,
+                         temperature=1.0):
+    """Overwrites ``X.shadow`` with the gradient of sum(logp * logp.shadow) + sum(entropy * entropy.shadow); ``entropy.primal`` and
+    ``checkpoints`` are the forward's.  ``X.shadow`` has X's row stride and may be X itself."""
+    pX = X.primal
+    M, N, ld = _logits(pX)
+    dl, pe, de = _logprob_weights(logp, targets, entropy, pX, N)
+    _logit_grad(pX, X.shadow, ld)
+    _row_array("checkpoints.M", checkpoints.M, (N,), torch.float32, pX)
+    _row_array("checkpoints.L", checkpoints.L, (N,), torch.float32, pX)
+    with _on(pX):
+        _check(_lib.tylo_b200_token_logprobs_bwd(_p(X.shadow), _p(dl), _p(de), _p(pX), _p(targets), _p(pe), _p(checkpoints.M),
+                                                 _p(checkpoints.L), M, N, ld, float(temperature), _dtype(pX), _stream()))
+
+
+def grad_token_logprobs(dlogp, X, targets, *, checkpoints, entropy=None, d_entropy=None, temperature=1.0):
+    """-> the gradient of X; ``entropy`` (the forward's) goes with ``d_entropy``."""
+    Xd = Duplicated(X, _like_logits(X, _logits(X)[2]))
+    grad_token_logprobs_(None if dlogp is None else Duplicated(dlogp, dlogp), Xd, targets, checkpoints=checkpoints,
+                         entropy=None if d_entropy is None else Duplicated(entropy, d_entropy), temperature=temperature)
+    return Xd.shadow
+
+
+def token_logprobs_with_grad_(logp: Optional[Duplicated], X: Duplicated, targets, *, entropy: Optional[Duplicated] = None, temperature=1.0):
+    """``token_logprobs_`` and ``grad_token_logprobs_`` in one launch, for weights (``logp.shadow``, ``entropy.shadow``) that are known
+    before the forward, as in next-token training.  Writes ``logp.primal``, ``entropy.primal`` and ``X.shadow`` (which may be X)."""
+    pX = X.primal
+    M, N, ld = _logits(pX)
+    dl, pe, de = _logprob_weights(logp, targets, entropy, pX, N)
+    pl = None if logp is None else logp.primal
+    _row_array("logp", pl, (N,), torch.float32, pX)
+    _logit_grad(pX, X.shadow, ld)
+    with _on(pX):
+        _check(_lib.tylo_b200_token_logprobs_fwd_bwd(_p(pl), _p(pe), _p(X.shadow), _p(dl), _p(de), _p(pX), _p(targets), M, N, ld,
+                                                     float(temperature), _dtype(pX), _stream()))
+
+
+def _distill_args(X, teacher, index, temperature, teacher_temperature, renormalize):
+    M, N, ld = _logits(X)
+    K = int(teacher.shape[-1])
+    _row_array("teacher", teacher, (N, K), torch.float32, X)
+    _row_array("index", index, (N, K), torch.int32, X)
+    u = temperature if teacher_temperature is None else teacher_temperature
+    return N, ld, K, (K, M, N, ld, float(temperature), float(u), int(bool(renormalize)), _dtype(X))
+
+
+def distill_(loss, X, teacher, index, *, temperature=1.0, teacher_temperature=None, renormalize=True, checkpoints=None):
+    """Distillation from a teacher's top logits: loss (N,) fp32 = sum_k P_k (log P_k - log softmax(X / temperature)[index_k]).
+    ``teacher`` (N, K) fp32 and ``index`` (N, K) int32: K entries per row in any order; with ``renormalize`` P is the softmax of
+    teacher / teacher_temperature over the row's entries, otherwise its exponential as it is.  ``teacher_temperature`` defaults to
+    ``temperature``; the alternatives of ``token_logprobs_`` already have theirs in them, so they go with 1.  Entries with an
+    index outside [0, M) are left out."""
+    pX, pl = primal(X), primal(loss)
+    N, ld, K, args = _distill_args(pX, teacher, index, temperature, teacher_temperature, renormalize)
+    _row_array("loss", pl, (N,), torch.float32, pX)
+    cm = cl = None
+    if checkpoints is not None:
+        cm, cl = checkpoints
+        _row_array("checkpoints.M", cm, (N,), torch.float32, pX)
+        _row_array("checkpoints.L", cl, (N,), torch.float32, pX)
+    with _on(pX):
+        _check(_lib.tylo_b200_distill_fwd(_p(pl), _p(cm), _p(cl), _p(pX), _p(teacher), _p(index), *args, _stream()))
+    return loss
+
+
+def distill(X, teacher, index, **kw):
+    loss = torch.empty(X.shape[0], dtype=torch.float32, device=X.device)
+    distill_(loss, X, teacher, index, **kw)
+    return loss
+
+
+def grad_distill_(loss: Duplicated, X: Duplicated, teacher, index, *, checkpoints, temperature=1.0, teacher_temperature=None,
+                  renormalize=True):
+    """Overwrites ``X.shadow`` with the gradient of sum(loss * loss.shadow); ``checkpoints`` are the forward's.  ``X.shadow`` has
+    X's row stride and may be X itself.  The teacher's entries are constants."""
+    pX = X.primal
+    N, ld, K, args = _distill_args(pX, teacher, index, temperature, teacher_temperature, renormalize)
+    _row_array("the loss's weights", loss.shadow, (N,), torch.float32, pX)
+    _logit_grad(pX, X.shadow, ld)
+    _row_array("checkpoints.M", checkpoints.M, (N,), torch.float32, pX)
+    _row_array("checkpoints.L", checkpoints.L, (N,), torch.float32, pX)
+    with _on(pX):
+        _check(_lib.tylo_b200_distill_bwd(_p(X.shadow), _p(loss.shadow), _p(pX), _p(teacher), _p(index), _p(checkpoints.M),
+                                          _p(checkpoints.L), *args, _stream()))
+
+
+def grad_distill(dloss, X, teacher, index, *, checkpoints, **kw):
+    """-> the gradient of X."""
+    Xd = Duplicated(X, _like_logits(X, _logits(X)[2]))
+    grad_distill_(Duplicated(dloss, dloss), Xd, teacher, index, checkpoints=checkpoints, **kw)
+    return Xd.shadow
+
+
+def distill_with_grad_(loss: Duplicated, X: Duplicated, teacher, index, *, temperature=1.0, teacher_temperature=None, renormalize=True):
+    """``distill_`` and ``grad_distill_`` in one launch, for weights (``loss.shadow``) that are known before the forward.  Writes
+    ``loss.primal`` and ``X.shadow`` (which may be X)."""
+    pX = X.primal
+    N, ld, K, args = _distill_args(pX, teacher, index, temperature, teacher_temperature, renormalize)
+    _row_array("loss", loss.primal, (N,), torch.float32, pX)
+    _row_array("the loss's weights", loss.shadow, (N,), torch.float32, pX)
+    _logit_grad(pX, X.shadow, ld)
+    with _on(pX):
+        _check(_lib.tylo_b200_distill_fwd_bwd(_p(loss.primal), _p(X.shadow), _p(loss.shadow), _p(pX), _p(teacher), _p(index), *args,
+                                              _stream()))
 
 
 # ---------------------------------------------------------------------------------------------

@@ -7,7 +7,7 @@ module ChainRulesCoreExt
 using Tylo
 import Tylo: shadow, _flex_attention, grad_shadow, ScoreMod
 using ChainRulesCore
-import ChainRulesCore: rrule, unthunk, NoTangent, Tangent
+import ChainRulesCore: rrule, unthunk, NoTangent, AbstractZero, Tangent
 
 function rrule(::typeof(rms_norm), X, W; eps, offset = 0.0f0)
     cp = allocate_checkpoints(rms_norm!, X, W)
@@ -43,6 +43,30 @@ function rrule(::typeof(softmax), X)
         return NoTangent(), shadow(Xd)
     end
     return Y, pullback
+end
+
+# the alternatives are a report: no gradient runs through them; the cotangent of a value that is not used is a zero tangent
+function rrule(::typeof(token_logprobs), X, targets; temperature = 1, entropy = false, top = 0)
+    cp = allocate_checkpoints(token_logprobs!, X)
+    out = token_logprobs(X, targets; temperature, entropy, top, checkpoints = cp)
+    function pullback(Ȳ)
+        Ȳ = unthunk(Ȳ)
+        l̄ = targets === nothing ? NoTangent() : unthunk(Ȳ.logp)
+        ē = entropy ? unthunk(Ȳ.entropy) : NoTangent()
+        l̄ isa AbstractZero && ē isa AbstractZero && return NoTangent(), NoTangent(), NoTangent()
+        given(x) = x isa AbstractZero ? nothing : x
+        X̄ = ∇token_logprobs(given(l̄), X, l̄ isa AbstractZero ? nothing : targets; checkpoints = cp, entropy = out.entropy, ē = given(ē),
+                            temperature)
+        return NoTangent(), X̄, NoTangent()
+    end
+    return out, pullback
+end
+
+function rrule(::typeof(distill), X, teacher, index; kwargs...)
+    cp = allocate_checkpoints(distill!, X)
+    loss = distill(X, teacher, index; checkpoints = cp, kwargs...)
+    pullback(loss̄) = (NoTangent(), ∇distill(unthunk(loss̄), X, teacher, index; checkpoints = cp, kwargs...), NoTangent(), NoTangent())
+    return loss, pullback
 end
 
 function rrule(::typeof(attention), Q, K, V; causal = false, kwargs...)

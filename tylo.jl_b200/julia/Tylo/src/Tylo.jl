@@ -19,6 +19,8 @@ include("attention/flex.jl")
 include("attention/attention.jl")
 include("attention/decode.jl")
 include("softmax/softmax.jl")
+include("vocab/logprobs.jl")
+include("vocab/distill.jl")
 include("norm/rms_norm.jl")
 include("norm/layer_norm.jl")
 

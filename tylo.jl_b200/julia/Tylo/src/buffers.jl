@@ -27,7 +27,7 @@ Duplicated(x) = Duplicated(x, similar(x))
     allocate_checkpoints(f!, args...) -> NamedTuple
 
 Saved activations that bridge `f!` and `∇f!` (`(; M, L)` for attention, `(; Rstd)` for RMSNorm,
-`(; Mean, Rstd)` for LayerNorm); always `Float32`.  Pass as the `checkpoints` keyword.
+`(; Mean, Rstd)` for LayerNorm, `(; M, L)` for `token_logprobs!` and `distill!`); always `Float32`.  Pass as the `checkpoints` keyword.
 """
 function allocate_checkpoints end
 
