@@ -61,7 +61,7 @@ __device__ __forceinline__ float teacher_row(const DistillArgs& a, size_t row, f
 template <typename T, bool LOSS, bool GRAD>
 __global__ void __launch_bounds__(kDistillThreads) distill_row_kernel(const DistillArgs a) {
   constexpr int VEC = Elem<T>::kVec, THREADS = kDistillThreads;
-  __shared__ float scratch[96];
+  __shared__ float scratch[100];
   __shared__ float p[TYLO_DISTILL_MAX], xk[TYLO_DISTILL_MAX];
   __shared__ int index[TYLO_DISTILL_MAX];
   const size_t row = blockIdx.x;
@@ -72,7 +72,10 @@ __global__ void __launch_bounds__(kDistillThreads) distill_row_kernel(const Dist
   const float log_norm = teacher_row<THREADS>(a, row, p, index, scratch, mass);
   for (int k = threadIdx.x; k < a.K; k += THREADS) xk[k] = index[k] >= 0 ? Elem<T>::to_f(x[index[k]]) : 0.f;
   VocabStats st;
-  if constexpr (LOSS) st = vocab_row_stats<T, THREADS, false>(x, r, scale, scratch);
+  if constexpr (LOSS) {
+    st = vocab_thread_stats<T, THREADS, 4, false>(x, r, VocabPart(0, 1, r.whole), scale);
+    vocab_reduce<THREADS>(st, scale, scratch, 1);
+  }
   else st = {a.inMx[row], a.inL[row], 0.f};
   const float mo = st.m == -INFINITY ? 0.f : st.m;
   if constexpr (LOSS) {

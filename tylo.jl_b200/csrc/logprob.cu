@@ -64,10 +64,10 @@ __device__ __forceinline__ void logprob_row_grad(T* dx, const T* x, const VocabR
   }
 }
 
-template <typename T, bool GRAD>
+template <typename T, bool ENTROPY, bool GRAD>
 __global__ void __launch_bounds__(kLogprobThreads) logprob_row_kernel(const LogprobArgs a) {
   constexpr int VEC = Elem<T>::kVec;
-  __shared__ float scratch[96];
+  __shared__ float scratch[100];
   __shared__ uint64_t keys[32];
   const size_t row = blockIdx.x;
   const T* x = (const T*)a.X + row * a.ldx;
@@ -76,7 +76,8 @@ __global__ void __launch_bounds__(kLogprobThreads) logprob_row_kernel(const Logp
   const int target = a.targets ? a.targets[row] : -1;
   const bool has = target >= 0 && target < a.M;
   const float xt = has ? Elem<T>::to_f(x[target]) : 0.f;
-  const VocabStats st = vocab_row_stats<T, kLogprobThreads, true>(x, r, scale, scratch);
+  VocabStats st = vocab_thread_stats<T, kLogprobThreads, 4, ENTROPY>(x, r, VocabPart(0, 1, r.whole), scale);
+  vocab_reduce<kLogprobThreads>(st, scale, scratch, 1);
   const float logL = st.s == 0.f ? 0.f : logf(st.s), H = st.s == 0.f ? 0.f : logL - kVocabLn2 * st.a / st.s;
   const float mo = st.m == -INFINITY ? 0.f : st.m;
   if (threadIdx.x == 0) {
@@ -144,7 +145,10 @@ extern "C" int32_t tylo_b200_token_logprobs_fwd(float* Logp, float* Entropy, flo
   LogprobArgs a = {};
   a.X = X; a.targets = targets; a.Logp = Logp; a.Entropy = Entropy; a.TopLogp = TopLogp; a.TopIndex = TopIndex; a.Mx = Mx; a.L = L;
   a.ldx = ldx; a.M = (int)M; a.top = top; a.temperature = temperature;
-  TYLO_DISPATCH_DTYPE(dtype, T, (logprob_row_kernel<T, false><<<(unsigned)N, kLogprobThreads, 0, (cudaStream_t)stream>>>(a)));
+  TYLO_DISPATCH_DTYPE(dtype, T, {
+    if (Entropy) logprob_row_kernel<T, true, false><<<(unsigned)N, kLogprobThreads, 0, (cudaStream_t)stream>>>(a);
+    else logprob_row_kernel<T, false, false><<<(unsigned)N, kLogprobThreads, 0, (cudaStream_t)stream>>>(a);
+  });
   return check_launch(who);
 }
 
@@ -182,6 +186,9 @@ extern "C" int32_t tylo_b200_token_logprobs_fwd_bwd(float* Logp, float* Entropy,
   LogprobArgs a = {};
   a.X = X; a.targets = targets; a.Logp = Logp; a.Entropy = Entropy; a.dX = dX; a.dLogp = dLogp; a.dEntropy = dEntropy;
   a.ldx = ldx; a.M = (int)M; a.temperature = temperature;
-  TYLO_DISPATCH_DTYPE(dtype, T, (logprob_row_kernel<T, true><<<(unsigned)N, kLogprobThreads, 0, (cudaStream_t)stream>>>(a)));
+  TYLO_DISPATCH_DTYPE(dtype, T, {
+    if (Entropy || dEntropy) logprob_row_kernel<T, true, true><<<(unsigned)N, kLogprobThreads, 0, (cudaStream_t)stream>>>(a);
+    else logprob_row_kernel<T, false, true><<<(unsigned)N, kLogprobThreads, 0, (cudaStream_t)stream>>>(a);
+  });
   return check_launch(who);
 }
