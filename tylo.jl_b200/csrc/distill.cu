@@ -23,8 +23,6 @@ struct DistillArgs {
   float temperature, teacher_temperature;
 };
 
-constexpr int kDistillThreads = 512;
-
 // The teacher's probabilities of a row into shared memory (-1 as the index of an entry that is left out); returns the normaliser's
 // logarithm, so that log p_k = v_k / u - the result, and P through `mass`.
 template <int THREADS>
@@ -58,27 +56,25 @@ __device__ __forceinline__ float teacher_row(const DistillArgs& a, size_t row, f
   return log_norm;
 }
 
-template <typename T, bool LOSS, bool GRAD>
-__global__ void __launch_bounds__(kDistillThreads) distill_row_kernel(const DistillArgs a) {
-  constexpr int VEC = Elem<T>::kVec, THREADS = kDistillThreads;
+template <typename T, int THREADS, bool LOSS, bool GRAD>
+__global__ void __launch_bounds__(THREADS) distill_row_kernel(const DistillArgs a, int parts) {
   __shared__ float scratch[100];
   __shared__ float p[TYLO_DISTILL_MAX], xk[TYLO_DISTILL_MAX];
   __shared__ int index[TYLO_DISTILL_MAX];
-  const size_t row = blockIdx.x;
+  const size_t row = blockIdx.x / parts;
   const T* x = (const T*)a.X + row * a.ldx;
   const VocabRow<T> r(x, a.M);
+  const VocabPart part(blockIdx.x % parts, parts, r.whole);
   const float it = 1.f / a.temperature, scale = kVocabLog2e / a.temperature;
+  VocabStats st;
+  if constexpr (LOSS) st = vocab_thread_stats<T, THREADS, 4, false>(x, r, part, scale);
   float mass;
   const float log_norm = teacher_row<THREADS>(a, row, p, index, scratch, mass);
   for (int k = threadIdx.x; k < a.K; k += THREADS) xk[k] = index[k] >= 0 ? Elem<T>::to_f(x[index[k]]) : 0.f;
-  VocabStats st;
-  if constexpr (LOSS) {
-    st = vocab_thread_stats<T, THREADS, 4, false>(x, r, VocabPart(0, 1, r.whole), scale);
-    vocab_reduce<THREADS>(st, scale, scratch, 1);
-  }
+  if constexpr (LOSS) vocab_reduce<THREADS>(st, scale, scratch, parts);
   else st = {a.inMx[row], a.inL[row], 0.f};
   const float mo = st.m == -INFINITY ? 0.f : st.m;
-  if constexpr (LOSS) {
+  if (LOSS && part.part == 0) {
     const float logL = st.s == 0.f ? 0.f : logf(st.s);
     float loss = 0.f;
     for (int k = threadIdx.x; k < a.K; k += THREADS)
@@ -95,30 +91,41 @@ __global__ void __launch_bounds__(kDistillThreads) distill_row_kernel(const Dist
     const float w = a.dLoss[row] * it;
     const bool none = w == 0.f || mass == 0.f || st.s == 0.f;
     const float c = none ? 0.f : w * mass / st.s;
-    auto grad = [&](float f) { return none ? 0.f : vocab_ex2((f - mo) * scale) * c; };
-    __syncthreads();             // xk is read before any gradient is written: dX may be X
-    const int one = r.single(threadIdx.x);
-    if (one >= 0) dx[one] = Elem<T>::from_f(grad(Elem<T>::to_f(x[one])));
-    for (int v = threadIdx.x; v < r.whole; v += THREADS) {
-      Pack<T> q;
-      q.raw = ld_logits(x + r.index(v));
-      float f[VEC];
-      q.unpack(f);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) f[j] = grad(f[j]);
-      q.pack(f);
-      st_stream(dx + r.index(v), q.raw);
-    }
+    auto grad = [&](float2 f) {
+      const float2 y = __fmul2_rn(__fadd2_rn(f, make_float2(-mo, -mo)), make_float2(scale, scale));
+      const float2 d = __fmul2_rn(make_float2(vocab_ex2(y.x), vocab_ex2(y.y)), make_float2(c, c));
+      return none ? make_float2(0.f, 0.f) : d;
+    };
+    if (!LOSS) __syncthreads();             // xk is read before any gradient is written: dX may be X
+    vocab_rewrite<T, THREADS, 4>(dx, x, r, part, -1, 0.f, grad);
     __syncthreads();
-    // the teacher's entries: every copy of an index sums all its copies in the same order and stores the same value
+    // the teacher's entries in this part: every copy of an index sums all its copies in the same order and stores the same value
     if (!none)
       for (int k = threadIdx.x; k < a.K; k += THREADS) {
         const int j = index[k];
-        if (j < 0) continue;
+        if (j < 0 || !part.holds(r, j)) continue;
         float sum = 0.f;
         for (int i = 0; i < a.K; ++i) sum += index[i] == j ? p[i] : 0.f;
-        dx[j] = Elem<T>::from_f(grad(xk[k]) - w * sum);
+        dx[j] = Elem<T>::from_f(grad(make_float2(xk[k], 0.f)).x - w * sum);
       }
+  }
+  if constexpr (LOSS) cluster_done(parts);
+}
+
+template <typename T, bool LOSS, bool GRAD>
+static int32_t distill_dispatch(const char* who, const DistillArgs& a, int64_t N, cudaStream_t stream) {
+  const int64_t packets = a.M / Elem<T>::kVec;
+  constexpr int LONG = GRAD && LOSS ? 1024 : 512;
+  if constexpr (!LOSS) {       // nothing to tell one another: plain CTAs, as many per row as fill the GPU several times over
+    int parts = 1;
+    while (parts < 64 && N * parts < 16 * sm_count() && packets >= 8LL * parts * LONG) parts *= 2;
+    if (packets <= 1024) distill_row_kernel<T, 128, LOSS, GRAD><<<(unsigned)N, 128, 0, stream>>>(a, 1);
+    else distill_row_kernel<T, LONG, LOSS, GRAD><<<(unsigned)(N * parts), LONG, 0, stream>>>(a, parts);
+    return check_launch(who);
+  } else {
+    if (packets <= 1024)
+      return launch_vocab(who, distill_row_kernel<T, 128, LOSS, GRAD>, a, N, vocab_parts(N, packets, 128), 128, stream);
+    return launch_vocab(who, distill_row_kernel<T, LONG, LOSS, GRAD>, a, N, vocab_parts(N, packets, LONG), LONG, stream);
   }
 }
 
@@ -153,8 +160,8 @@ extern "C" int32_t tylo_b200_distill_fwd(float* Loss, float* Mx, float* L, const
   TYLO_REQUIRE(!Mx == !L, TYLO_ERR_INVALID_ARGUMENT, "%s: checkpoints Mx and L go together", who);
   DistillArgs a = distill_args(X, teacher, index, K, M, ldx, temperature, teacher_temperature, renormalize);
   a.Loss = Loss; a.Mx = Mx; a.L = L;
-  TYLO_DISPATCH_DTYPE(dtype, T, (distill_row_kernel<T, true, false><<<(unsigned)N, kDistillThreads, 0, (cudaStream_t)stream>>>(a)));
-  return check_launch(who);
+  TYLO_DISPATCH_DTYPE(dtype, T, return (distill_dispatch<T, true, false>(who, a, N, (cudaStream_t)stream)));
+  return TYLO_OK;
 }
 
 extern "C" int32_t tylo_b200_distill_bwd(void* dX, const float* dLoss, const void* X, const float* teacher, const int32_t* index,
@@ -168,8 +175,8 @@ extern "C" int32_t tylo_b200_distill_bwd(void* dX, const float* dLoss, const voi
   TYLO_REQUIRE(Mx && L, TYLO_ERR_INVALID_ARGUMENT, "%s: checkpoints Mx and L from the forward are required", who);
   DistillArgs a = distill_args(X, teacher, index, K, M, ldx, temperature, teacher_temperature, renormalize);
   a.dX = dX; a.dLoss = dLoss; a.inMx = Mx; a.inL = L;
-  TYLO_DISPATCH_DTYPE(dtype, T, (distill_row_kernel<T, false, true><<<(unsigned)N, kDistillThreads, 0, (cudaStream_t)stream>>>(a)));
-  return check_launch(who);
+  TYLO_DISPATCH_DTYPE(dtype, T, return (distill_dispatch<T, false, true>(who, a, N, (cudaStream_t)stream)));
+  return TYLO_OK;
 }
 
 extern "C" int32_t tylo_b200_distill_fwd_bwd(float* Loss, void* dX, const float* dLoss, const void* X, const float* teacher,
@@ -181,6 +188,6 @@ extern "C" int32_t tylo_b200_distill_fwd_bwd(float* Loss, void* dX, const float*
   TYLO_REQUIRE(aligned16(dX), TYLO_ERR_MISALIGNED, "%s: dX must be 16-byte aligned", who);
   DistillArgs a = distill_args(X, teacher, index, K, M, ldx, temperature, teacher_temperature, renormalize);
   a.Loss = Loss; a.dX = dX; a.dLoss = dLoss;
-  TYLO_DISPATCH_DTYPE(dtype, T, (distill_row_kernel<T, true, true><<<(unsigned)N, kDistillThreads, 0, (cudaStream_t)stream>>>(a)));
-  return check_launch(who);
+  TYLO_DISPATCH_DTYPE(dtype, T, return (distill_dispatch<T, true, true>(who, a, N, (cudaStream_t)stream)));
+  return TYLO_OK;
 }

@@ -19,111 +19,110 @@ struct LogprobArgs {
   float temperature;
 };
 
-constexpr int kLogprobThreads = 512;
-
-__device__ __forceinline__ uint64_t block_max_key(uint64_t k, uint64_t* scratch) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const uint64_t k2 = __shfl_xor_sync(0xffffffffu, k, o);
-    k = k2 > k ? k2 : k;
+// What a row's gradient needs: dX_j = e_j (A y_j + B) with e_j = exp2(y_j), y_j in units of log 2, and `at` at the target.
+struct LogprobGrad {
+  float mo, scale, A, B, at;
+  bool none;
+  __device__ __forceinline__ LogprobGrad(float mx, float L, float g, float h, float H, float temperature) {
+    const float it = 1.f / temperature, inv = 1.f / L;
+    none = (g == 0.f && h == 0.f) || L == 0.f;
+    mo = mx == -INFINITY ? 0.f : mx;
+    scale = kVocabLog2e * it;
+    // -p (g + h (log p + H)) / t with log p = ln 2 (y - log2 L)
+    A = -h * kVocabLn2 * it * inv;
+    B = -(g + (h == 0.f ? 0.f : h * (H - logf(L)))) * it * inv;
+    at = none ? 0.f : g * it;
   }
-  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = k;
-  __syncthreads();
-  k = 0;
-  for (int w = 0; w < kLogprobThreads / 32; ++w) k = scratch[w] > k ? scratch[w] : k;
-  __syncthreads();
-  return k;
-}
-
-// Writes the gradient of a row: p (c0 + c1 log2 p) per element, c0 = -(g + h H) / t, c1 = -h ln 2 / t, and g / t at the target.
-template <typename T>
-__device__ __forceinline__ void logprob_row_grad(T* dx, const T* x, const VocabRow<T>& r, int first, int step, int last, bool singles,
-                                                 int target, float mx, float L, float g, float h, float H, float temperature) {
-  constexpr int VEC = Elem<T>::kVec;
-  const float it = 1.f / temperature, scale = kVocabLog2e * it;
-  const bool none = (g == 0.f && h == 0.f) || L == 0.f;
-  const float mo = mx == -INFINITY ? 0.f : mx, inv = 1.f / L, lg = log2f(L);
-  const float c0 = -(h == 0.f ? g : g + h * H) * it, c1 = -h * kVocabLn2 * it, at = g * it;
-  auto grad = [&](float f, int j) {
-    const float y = (f - mo) * scale, p = vocab_ex2(y) * inv;
-    float d = p * fmaf(c1, fmaxf(y, kExpFloor) - lg, c0);
-    if (j == target) d += at;
-    return none ? 0.f : d;
-  };
-  const int one = r.single(threadIdx.x);
-  if (singles && one >= 0) dx[one] = Elem<T>::from_f(grad(Elem<T>::to_f(x[one]), one));
-  for (int v = first; v < last; v += step) {
-    Pack<T> p;
-    p.raw = ld_logits(x + r.index(v));
-    float f[VEC];
-    p.unpack(f);
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) f[j] = grad(f[j], r.index(v) + j);
-    p.pack(f);
-    st_stream(dx + r.index(v), p.raw);
+  template <bool ENTROPY> __device__ __forceinline__ float2 operator()(float2 x) const {
+    const float2 y = __fmul2_rn(__fadd2_rn(x, make_float2(-mo, -mo)), make_float2(scale, scale));
+    const float2 e = make_float2(vocab_ex2(y.x), vocab_ex2(y.y));
+    float2 d;
+    if constexpr (ENTROPY)
+      d = __fmul2_rn(e, __ffma2_rn(make_float2(A, A), make_float2(fmaxf(y.x, kExpFloor), fmaxf(y.y, kExpFloor)), make_float2(B, B)));
+    else
+      d = __fmul2_rn(e, make_float2(B, B));
+    return none ? make_float2(0.f, 0.f) : d;
   }
-}
+};
 
-template <typename T, bool ENTROPY, bool GRAD>
-__global__ void __launch_bounds__(kLogprobThreads) logprob_row_kernel(const LogprobArgs a) {
-  constexpr int VEC = Elem<T>::kVec;
+template <typename T, int THREADS, bool ENTROPY, bool TOP, bool GRAD>
+__global__ void __launch_bounds__(THREADS) logprob_row_kernel(const LogprobArgs a, int parts) {
   __shared__ float scratch[100];
-  __shared__ uint64_t keys[32];
-  const size_t row = blockIdx.x;
+  const size_t row = blockIdx.x / parts;
   const T* x = (const T*)a.X + row * a.ldx;
   const VocabRow<T> r(x, a.M);
+  const VocabPart part(blockIdx.x % parts, parts, r.whole);
   const float scale = kVocabLog2e / a.temperature;
   const int target = a.targets ? a.targets[row] : -1;
   const bool has = target >= 0 && target < a.M;
   const float xt = has ? Elem<T>::to_f(x[target]) : 0.f;
-  VocabStats st = vocab_thread_stats<T, kLogprobThreads, 4, ENTROPY>(x, r, VocabPart(0, 1, r.whole), scale);
-  vocab_reduce<kLogprobThreads>(st, scale, scratch, 1);
+  VocabStats st = vocab_thread_stats<T, THREADS, 4, ENTROPY>(x, r, part, scale);
+  uint32_t mine = 0;
+  if constexpr (TOP) mine = vocab_mine<T, THREADS>(x, r, part, st);
+  vocab_reduce<THREADS>(st, scale, scratch, parts);
   const float logL = st.s == 0.f ? 0.f : logf(st.s), H = st.s == 0.f ? 0.f : logL - kVocabLn2 * st.a / st.s;
   const float mo = st.m == -INFINITY ? 0.f : st.m;
-  if (threadIdx.x == 0) {
+  if (threadIdx.x == 0 && part.part == 0) {
     if (a.Logp) a.Logp[row] = has ? (xt - mo) / a.temperature - logL : 0.f;
     if (a.Entropy) a.Entropy[row] = H;
     if (a.Mx) { a.Mx[row] = st.m; a.L[row] = st.s; }
   }
-  uint64_t below = ~0ull;
-  for (int k = 0; k < a.top; ++k) {
-    uint64_t best = 0;
-    const int one = r.single(threadIdx.x);
-    if (one >= 0) {
-      const uint64_t key = vocab_key(Elem<T>::to_f(x[one]), one);
-      if (key < below) best = key;
-    }
-    for (int v = threadIdx.x; v < r.whole; v += kLogprobThreads) {
-      Pack<T> p;
-      p.raw = ld_logits(x + r.index(v));
-      float f[VEC];
-      p.unpack(f);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const uint64_t key = vocab_key(f[j], r.index(v) + j);
-        if (key < below && key > best) best = key;
-      }
-    }
-    below = block_max_key(best, keys);
-    if (threadIdx.x == 0) {
-      a.TopLogp[row * a.top + k] = (vocab_unkey((uint32_t)(below >> 32)) - mo) / a.temperature - logL;
-      a.TopIndex[row * a.top + k] = vocab_key_index(below);
-    }
+  if constexpr (TOP) {
+    __shared__ TopScratch<THREADS> top;
+    const int n = vocab_top<T, THREADS>(x, r, part, a.top, mine, top);
+    vocab_ranked<THREADS>(top, n, a.top, parts, [&](int rank, uint64_t key) {
+      a.TopLogp[row * a.top + rank] = (vocab_unkey((uint32_t)(key >> 32)) - mo) / a.temperature - logL;
+      a.TopIndex[row * a.top + rank] = vocab_key_index(key);
+    });
   }
-  if constexpr (GRAD)
-    logprob_row_grad<T>((T*)a.dX + row * a.ldx, x, r, threadIdx.x, kLogprobThreads, r.whole, true, has ? target : -1, st.m, st.s,
-                        has ? a.dLogp[row] : 0.f, a.dEntropy ? a.dEntropy[row] : 0.f, H, a.temperature);
+  if constexpr (GRAD) {
+    const LogprobGrad d(st.m, st.s, has ? a.dLogp[row] : 0.f, a.dEntropy ? a.dEntropy[row] : 0.f, H, a.temperature);
+    vocab_rewrite<T, THREADS, 4>((T*)a.dX + row * a.ldx, x, r, part, has ? target : -1, d.at,
+                                 [&](float2 f) { return d.template operator()<ENTROPY>(f); });
+  }
+  cluster_done(parts);
+}
+
+template <typename T, int THREADS, bool ENTROPY>
+__global__ void __launch_bounds__(THREADS) logprob_bwd_kernel(const LogprobArgs a, int parts) {
+  const size_t row = blockIdx.x / parts;
+  const T* x = (const T*)a.X + row * a.ldx;
+  const VocabRow<T> r(x, a.M);
+  const VocabPart part(blockIdx.x % parts, parts, r.whole);
+  const int target = a.targets ? a.targets[row] : -1;
+  const bool has = target >= 0 && target < a.M;
+  const LogprobGrad d(a.inMx[row], a.inL[row], has ? a.dLogp[row] : 0.f, ENTROPY ? a.dEntropy[row] : 0.f, ENTROPY ? a.inEntropy[row] : 0.f,
+                      a.temperature);
+  vocab_rewrite<T, THREADS, 4>((T*)a.dX + row * a.ldx, x, r, part, has ? target : -1, d.at,
+                               [&](float2 f) { return d.template operator()<ENTROPY>(f); });
+}
+
+template <typename T, int THREADS, bool ENTROPY, bool GRAD>
+static int32_t logprob_launch(const char* who, const LogprobArgs& a, int64_t N, cudaStream_t stream) {
+  const int parts = vocab_parts(N, a.M / Elem<T>::kVec, THREADS);
+  if constexpr (!GRAD)
+    if (a.top) return launch_vocab(who, logprob_row_kernel<T, THREADS, ENTROPY, true, false>, a, N, parts, THREADS, stream);
+  return launch_vocab(who, logprob_row_kernel<T, THREADS, ENTROPY, false, GRAD>, a, N, parts, THREADS, stream);
+}
+
+template <typename T, bool GRAD>
+static int32_t logprob_dispatch(const char* who, const LogprobArgs& a, int64_t N, cudaStream_t stream) {
+  const bool entropy = a.Entropy || a.dEntropy;
+  constexpr int LONG = GRAD ? 1024 : 512;
+  if (a.M / Elem<T>::kVec <= 1024)
+    return entropy ? logprob_launch<T, 128, true, GRAD>(who, a, N, stream) : logprob_launch<T, 128, false, GRAD>(who, a, N, stream);
+  return entropy ? logprob_launch<T, LONG, true, GRAD>(who, a, N, stream) : logprob_launch<T, LONG, false, GRAD>(who, a, N, stream);
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kLogprobThreads) logprob_bwd_kernel(const LogprobArgs a) {
-  const size_t row = blockIdx.x;
-  const T* x = (const T*)a.X + row * a.ldx;
-  const VocabRow<T> r(x, a.M);
-  const int target = a.targets ? a.targets[row] : -1;
-  const bool has = target >= 0 && target < a.M;
-  logprob_row_grad<T>((T*)a.dX + row * a.ldx, x, r, threadIdx.x, kLogprobThreads, r.whole, true, has ? target : -1, a.inMx[row], a.inL[row],
-                      has ? a.dLogp[row] : 0.f, a.dEntropy ? a.dEntropy[row] : 0.f, a.dEntropy ? a.inEntropy[row] : 0.f, a.temperature);
+static int32_t logprob_bwd_dispatch(const char* who, const LogprobArgs& a, int64_t N, cudaStream_t stream) {
+  constexpr int THREADS = 256;
+  const int64_t packets = a.M / Elem<T>::kVec;
+  const int segments = (int)((packets + 4 * THREADS - 1) / (4 * THREADS));
+  const unsigned grid = (unsigned)(N * (segments > 0 ? segments : 1));
+  if (a.dEntropy) logprob_bwd_kernel<T, THREADS, true><<<grid, THREADS, 0, stream>>>(a, segments > 0 ? segments : 1);
+  else logprob_bwd_kernel<T, THREADS, false><<<grid, THREADS, 0, stream>>>(a, segments > 0 ? segments : 1);
+  return check_launch(who);
 }
 
 }  // namespace tylo
@@ -145,11 +144,8 @@ extern "C" int32_t tylo_b200_token_logprobs_fwd(float* Logp, float* Entropy, flo
   LogprobArgs a = {};
   a.X = X; a.targets = targets; a.Logp = Logp; a.Entropy = Entropy; a.TopLogp = TopLogp; a.TopIndex = TopIndex; a.Mx = Mx; a.L = L;
   a.ldx = ldx; a.M = (int)M; a.top = top; a.temperature = temperature;
-  TYLO_DISPATCH_DTYPE(dtype, T, {
-    if (Entropy) logprob_row_kernel<T, true, false><<<(unsigned)N, kLogprobThreads, 0, (cudaStream_t)stream>>>(a);
-    else logprob_row_kernel<T, false, false><<<(unsigned)N, kLogprobThreads, 0, (cudaStream_t)stream>>>(a);
-  });
-  return check_launch(who);
+  TYLO_DISPATCH_DTYPE(dtype, T, return (logprob_dispatch<T, false>(who, a, N, (cudaStream_t)stream)));
+  return TYLO_OK;
 }
 
 static int32_t check_logprob_grad(const char* who, const void* dX, const float* dLogp, const float* dEntropy, const int32_t* targets) {
@@ -172,8 +168,8 @@ extern "C" int32_t tylo_b200_token_logprobs_bwd(void* dX, const float* dLogp, co
   LogprobArgs a = {};
   a.X = X; a.targets = targets; a.dX = dX; a.dLogp = dLogp; a.dEntropy = dEntropy; a.inEntropy = Entropy; a.inMx = Mx; a.inL = L;
   a.ldx = ldx; a.M = (int)M; a.temperature = temperature;
-  TYLO_DISPATCH_DTYPE(dtype, T, (logprob_bwd_kernel<T><<<(unsigned)N, kLogprobThreads, 0, (cudaStream_t)stream>>>(a)));
-  return check_launch(who);
+  TYLO_DISPATCH_DTYPE(dtype, T, return (logprob_bwd_dispatch<T>(who, a, N, (cudaStream_t)stream)));
+  return TYLO_OK;
 }
 
 extern "C" int32_t tylo_b200_token_logprobs_fwd_bwd(float* Logp, float* Entropy, void* dX, const float* dLogp, const float* dEntropy,
@@ -186,9 +182,6 @@ extern "C" int32_t tylo_b200_token_logprobs_fwd_bwd(float* Logp, float* Entropy,
   LogprobArgs a = {};
   a.X = X; a.targets = targets; a.Logp = Logp; a.Entropy = Entropy; a.dX = dX; a.dLogp = dLogp; a.dEntropy = dEntropy;
   a.ldx = ldx; a.M = (int)M; a.temperature = temperature;
-  TYLO_DISPATCH_DTYPE(dtype, T, {
-    if (Entropy || dEntropy) logprob_row_kernel<T, true, true><<<(unsigned)N, kLogprobThreads, 0, (cudaStream_t)stream>>>(a);
-    else logprob_row_kernel<T, false, true><<<(unsigned)N, kLogprobThreads, 0, (cudaStream_t)stream>>>(a);
-  });
-  return check_launch(who);
+  TYLO_DISPATCH_DTYPE(dtype, T, return (logprob_dispatch<T, true>(who, a, N, (cudaStream_t)stream)));
+  return TYLO_OK;
 }

@@ -109,6 +109,11 @@ struct VocabPart {
     lo = min(part * per, whole);
     hi = min(lo + per, whole);
   }
+  template <typename R> __device__ __forceinline__ bool holds(const R& r, int index) const {
+    const int e = index - r.head;
+    if (e < 0 || e >= r.whole * R::kVec) return part == 0;
+    return e / R::kVec >= lo && e / R::kVec < hi;
+  }
 };
 
 // Largest element of U packets, a NaN passed over; 16-bit types two at a time.
@@ -199,6 +204,56 @@ __device__ __forceinline__ VocabStats vocab_thread_stats(const T* x, const Vocab
   return {m, s.x + s.y, a.x + a.y};
 }
 
+// Second look at a part: f(pair of logits) -> pair of gradients for every element, `at` added to element `hot`.  Rounded once, on the way out.
+template <typename T, int THREADS, int U, typename F>
+__device__ __forceinline__ void vocab_rewrite(T* dx, const T* x, const VocabRow<T>& r, const VocabPart& part, int hot, float at, F f) {
+  constexpr int VEC = Elem<T>::kVec;
+  const int one = part.part == 0 ? r.single(threadIdx.x) : -1;
+  if (one >= 0) dx[one] = Elem<T>::from_f(f(make_float2(Elem<T>::to_f(x[one]), 0.f)).x + (one == hot ? at : 0.f));
+  // packet and place of `hot`; -1 where it is a single element or not there
+  const int hv = hot >= r.head && hot < r.head + r.whole * VEC ? (hot - r.head) / VEC : -1, hj = (hot - r.head) % VEC;
+  x += r.head;
+  dx += r.head;
+  auto load = [&](Pack<T> (&p)[U], int v0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (v0 + u * THREADS < part.hi) p[u].raw = ld_logits(x + (size_t)(v0 + u * THREADS) * VEC);
+  };
+  auto give = [&](Pack<T> (&p)[U], int v0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int v = v0 + u * THREADS;
+      float e[VEC];
+      p[u].unpack(e);
+#pragma unroll
+      for (int j = 0; j < VEC; j += 2) {
+        const float2 d = f(make_float2(e[j], e[j + 1]));
+        e[j] = d.x; e[j + 1] = d.y;
+      }
+      if (v == hv) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) e[j] += j == hj ? at : 0.f;
+      }
+      p[u].pack(e);
+      if (v < part.hi) st_stream(dx + (size_t)v * VEC, p[u].raw);
+    }
+  };
+  int v0 = part.lo + threadIdx.x;
+  if (v0 >= part.hi) return;
+  Pack<T> p[U], q[U];
+  load(p, v0);
+  while (true) {
+    const int v1 = v0 + U * THREADS;
+    if (v1 >= part.hi) { give(p, v0); break; }
+    load(q, v1);
+    give(p, v0);
+    v0 = v1 + U * THREADS;
+    if (v0 >= part.hi) { give(q, v1); break; }
+    load(p, v0);
+    give(q, v1);
+  }
+}
+
 // Order of the alternatives as whole numbers: larger logits first, the lower index first among equals, a NaN above everything.
 // Zero stands for "no entry" (no logit maps to it).
 __device__ __forceinline__ uint32_t vocab_key(float x) {
@@ -213,6 +268,300 @@ __device__ __forceinline__ uint64_t vocab_key(float x, int index) {
   return ((uint64_t)vocab_key(x) << 32) | (uint32_t)(0x7fffffff - index);
 }
 __device__ __forceinline__ int vocab_key_index(uint64_t k) { return 0x7fffffff - (int)(uint32_t)k; }
+
+// ---- the largest elements of a part ------------------------------------------------------------------------------------------
+// A bound first: the K-th largest of the threads' own maxima, which the statistics leave behind, is no larger than the K-th largest
+// element, and no more than K threads (and ties) have anything to show above it.  Only those read their elements again, out of L2,
+// and put what reaches the bound into shared memory: little more than K elements unless they sit together in few threads' shares or
+// are equal.  Where they do not fit, the bound is raised by counting, and equal elements at the bound are taken in the order of
+// their index.  What is left is thinned by bisection to K and a few, whose rank is counted.
+constexpr int kTopSlack = 32;
+
+template <int THREADS> struct TopScratch {
+  static constexpr int kSlots = 8 * THREADS;
+  uint64_t keys[kSlots];
+  uint64_t few[TYLO_TOP_MAX + kTopSlack];
+  uint64_t sorted[TYLO_TOP_MAX];
+  uint32_t warp[64];
+  int n, m;
+};
+
+template <int THREADS> struct BlockCount {
+  // sum over the CTA; `buf` alternates between two halves so that one barrier per sum is enough
+  uint32_t* buf;
+  int half;
+  __device__ __forceinline__ int operator()(int c) {
+    c = __reduce_add_sync(0xffffffffu, c);
+    uint32_t* b = buf + 32 * half;
+    half ^= 1;
+    if ((threadIdx.x & 31) == 0) b[threadIdx.x >> 5] = c;
+    __syncthreads();
+    const int lane = threadIdx.x & 31;
+    return __reduce_add_sync(0xffffffffu, lane < THREADS / 32 ? (int)b[lane] : 0);
+  }
+};
+
+// Applies f(value, index) to the elements of this thread's share, in the share's order; `some(packet's values)` may skip a packet.
+template <typename T, int THREADS, typename S, typename F>
+__device__ __forceinline__ void vocab_share(const T* x, const VocabRow<T>& r, const VocabPart& part, S some, F f) {
+  constexpr int VEC = Elem<T>::kVec, U = 4;
+  const int one = part.part == 0 ? r.single(threadIdx.x) : -1;
+  if (one >= 0) f(Elem<T>::to_f(x[one]), one);
+  for (int v0 = part.lo + threadIdx.x; v0 < part.hi; v0 += U * THREADS) {
+    Pack<T> p[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (v0 + u * THREADS < part.hi) p[u].raw = ld_logits(x + r.index(v0 + u * THREADS));
+#pragma unroll 1
+    for (int u = 0; u < U; ++u) {
+      const int v = v0 + u * THREADS;
+      Pack<T> q = p[0];
+#pragma unroll
+      for (int w = 1; w < U; ++w)
+        if (w == u) q = p[w];
+      if (v >= part.hi) break;
+      float e[VEC];
+      q.unpack(e);
+      if (!some(e)) continue;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) f(e[j], r.index(v) + j);
+    }
+  }
+}
+
+// Puts the min(K, elements of the part) largest elements of the part into sc.sorted, in falling order, and returns how many.
+// `mine`: this thread's largest element as a key, 0 without elements.
+template <typename T, int THREADS>
+__device__ int vocab_top(const T* x, const VocabRow<T>& r, const VocabPart& part, int K, uint32_t mine, TopScratch<THREADS>& sc) {
+  constexpr int VEC = Elem<T>::kVec, kTopSlots = TopScratch<THREADS>::kSlots;
+  const int elements = (part.hi - part.lo) * VEC + (part.part == 0 ? r.head + r.tail : 0);
+  K = min(K, elements);
+  BlockCount<THREADS> count{sc.warp, 0};
+  if (threadIdx.x == 0) { sc.n = 0; sc.m = 0; }
+  const int lane = threadIdx.x & 31;
+  // largest and smallest key among the threads that have one
+  uint32_t hi = __reduce_max_sync(0xffffffffu, mine), lo = __reduce_min_sync(0xffffffffu, mine ? mine : 0xffffffffu);
+  if (lane == 0) { sc.warp[threadIdx.x >> 5] = hi; sc.warp[32 + (threadIdx.x >> 5)] = lo; }
+  __syncthreads();
+  hi = __reduce_max_sync(0xffffffffu, lane < THREADS / 32 ? sc.warp[lane] : 0);
+  lo = __reduce_min_sync(0xffffffffu, lane < THREADS / 32 ? sc.warp[32 + lane] : 0xffffffffu);
+  const uint32_t top = hi;
+  uint32_t t = 1;                              // below every element
+  if (__syncthreads_count(mine != 0) >= K) {
+    while (lo < hi) {
+      const uint32_t mid = lo + (hi - lo) / 2 + 1;
+      const int c = __syncthreads_count(mine >= mid);
+      if (c >= K) {
+        lo = mid;
+        if (c <= K + K / 8) break;
+      } else {
+        hi = mid - 1;
+      }
+    }
+    t = lo;
+  }
+  // elements above or at a bound; what does not fit is counted all the same
+  auto collect = [&](uint32_t from) {
+    const float low = from <= 1 ? -INFINITY : vocab_unkey(from);
+    if (mine >= from)
+      vocab_share<T, THREADS>(x, r, part, [&](const float (&e)[VEC]) {
+        bool any = false;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) any |= !(e[j] < low);
+        return any;
+      }, [&](float e, int j) {
+        if (vocab_key(e) >= from) {
+          const int at = atomicAdd(&sc.n, 1);
+          if (at < kTopSlots) sc.keys[at] = vocab_key(e, j);
+        }
+      });
+    __syncthreads();
+    const int n = sc.n;
+    __syncthreads();
+    return n;
+  };
+  auto at_least = [&](uint32_t from) {
+    int c = 0;
+    if (mine >= from)
+      vocab_share<T, THREADS>(x, r, part, [](const float (&)[VEC]) { return true; }, [&](float e, int) { c += vocab_key(e) >= from; });
+    return count(c);
+  };
+  auto clear = [&]() {
+    if (threadIdx.x == 0) sc.n = 0;
+    __syncthreads();
+  };
+  auto above = [&](uint32_t bound) { return bound == 0xffffffffu ? 0 : collect(bound + 1); };     // nothing is above a NaN
+  int n = collect(t);
+  if (n > kTopSlots) {
+    clear();
+    n = above(t);
+    if (n > kTopSlots) {                       // raise it: at_least(lo) >= K, at_least(hi + 1) < K
+      lo = t + 1; hi = top;
+      while (lo < hi) {
+        const uint32_t mid = lo + (hi - lo) / 2 + 1;
+        const int c = at_least(mid);
+        if (c >= K) {
+          lo = mid;
+          if (c <= kTopSlots) break;
+        } else {
+          hi = mid - 1;
+        }
+      }
+      t = lo;
+      clear();
+      n = collect(t);
+      if (n > kTopSlots) { clear(); n = above(t); }
+    }
+    if (n < K) {
+      // the elements equal to the bound, lowest index first: they are counted off in blocks of THREADS packets
+      const int need = K - n;
+      int taken = 0;
+      auto block = [&](uint32_t ties, int first) {        // bit j: element first + j
+        const int c = __popc(ties);
+        int before = c;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int up = __shfl_up_sync(0xffffffffu, before, o);
+          if (lane >= o) before += up;
+        }
+        if (lane == 31) sc.warp[threadIdx.x >> 5] = before;
+        __syncthreads();
+        int ahead = 0, all = 0;
+        for (int w = 0; w < THREADS / 32; ++w) {
+          const int k = sc.warp[w];
+          ahead += w < (int)(threadIdx.x >> 5) ? k : 0;
+          all += k;
+        }
+        __syncthreads();
+        int rank = taken + ahead + before - c;
+        for (uint32_t b = ties; b && rank < need; b &= b - 1, ++rank)
+          sc.keys[n + rank] = ((uint64_t)t << 32) | (uint32_t)(0x7fffffff - (first + __ffs(b) - 1));
+        taken += all;
+      };
+      if (part.part == 0 && r.head) block((int)threadIdx.x < r.head && vocab_key(Elem<T>::to_f(x[threadIdx.x])) == t, threadIdx.x);
+      for (int v0 = part.lo; v0 < part.hi && taken < need; v0 += THREADS) {
+        const int v = v0 + threadIdx.x;
+        uint32_t ties = 0;
+        if (v < part.hi) {
+          Pack<T> p;
+          p.raw = ld_logits(x + r.index(v));
+          float e[VEC];
+          p.unpack(e);
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) ties |= (uint32_t)(vocab_key(e[j]) == t) << j;
+        }
+        block(ties, r.index(v));
+      }
+      if (part.part == 0 && r.tail && taken < need)
+        block((int)threadIdx.x < r.tail && vocab_key(Elem<T>::to_f(x[r.M - r.tail + threadIdx.x])) == t, r.M - r.tail + threadIdx.x);
+      n = K;
+      __syncthreads();
+    }
+  }
+  // n >= K different keys: thin them, then rank them
+  const uint64_t* list = sc.keys;
+  if (n > K + kTopSlack) {
+    constexpr int PER = kTopSlots / THREADS;
+    uint64_t mine64[PER], most = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      mine64[i] = i * THREADS + threadIdx.x < n ? sc.keys[i * THREADS + threadIdx.x] : 0;
+      most = mine64[i] > most ? mine64[i] : most;
+    }
+    uint64_t lo64 = (uint64_t)t << 32, hi64 = ((uint64_t)top << 32) | 0xffffffffu;
+    while (lo64 < hi64) {
+      const uint64_t mid = lo64 + (hi64 - lo64) / 2 + 1;
+      int c = 0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (i * THREADS < n) c += __syncthreads_count(mine64[i] >= mid);
+      if (c >= K) {
+        lo64 = mid;
+        if (c <= K + kTopSlack) break;
+      } else {
+        hi64 = mid - 1;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (mine64[i] >= lo64) sc.few[atomicAdd(&sc.m, 1)] = mine64[i];
+    __syncthreads();
+    n = sc.m;
+    list = sc.few;
+  }
+  for (int i = threadIdx.x; i < n; i += THREADS) {
+    const uint64_t k = list[i];
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += list[j] > k;
+    if (rank < K) sc.sorted[rank] = k;
+  }
+  __syncthreads();
+  return K;
+}
+
+// Hands every one of the row's `K` largest elements to f(rank, key), whichever CTA of the row's cluster holds it: its rank is its place
+// in its own list and, for every other list, the number of larger elements there (lists are sorted: a binary search).
+template <int THREADS, typename F>
+__device__ __forceinline__ void vocab_ranked(TopScratch<THREADS>& sc, int n, int K, int parts, F f) {
+  if (parts > 1) {
+    if (threadIdx.x == 0) sc.m = n;
+    cg::this_cluster().sync();
+  }
+  for (int i = threadIdx.x; i < n; i += THREADS) {
+    const uint64_t k = sc.sorted[i];
+    int rank = i;
+    if (parts > 1) {
+      cg::cluster_group cluster = cg::this_cluster();
+      for (int c = 0; c < parts; ++c) {
+        if (c == (int)cluster.block_rank()) continue;
+        const TopScratch<THREADS>* peer = cluster.map_shared_rank(&sc, c);
+        int lo = 0, hi = peer->m;
+        while (lo < hi) {
+          const int mid = (lo + hi) / 2;
+          if (peer->sorted[mid] > k) lo = mid + 1; else hi = mid;
+        }
+        rank += lo;
+      }
+    }
+    if (rank < K) f(rank, k);
+  }
+}
+
+// This thread's largest element as a key; a NaN counts, so a share whose sum is NaN is looked through.
+template <typename T, int THREADS>
+__device__ __forceinline__ uint32_t vocab_mine(const T* x, const VocabRow<T>& r, const VocabPart& part, const VocabStats& st) {
+  uint32_t k = 0;
+  if (st.s != st.s) {
+    vocab_share<T, THREADS>(x, r, part, [](const float (&)[Elem<T>::kVec]) { return true; }, [&](float e, int) { k = max(k, vocab_key(e)); });
+  } else if (part.lo + (int)threadIdx.x < part.hi || (part.part == 0 && r.single(threadIdx.x) >= 0)) {
+    k = vocab_key(st.m);
+  }
+  return k;
+}
+
+// Launches `parts` CTAs per row, as a cluster where they have something to tell one another.
+template <typename A>
+int32_t launch_vocab(const char* who, void (*kernel)(A, int), const A& args, int64_t N, int parts, int threads, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(N * parts));
+  cfg.blockDim = dim3(threads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = parts; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = parts > 1 ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args, parts);
+  if (e != cudaSuccess) { set_error("launch of %s failed: %s", who, cudaGetErrorString(e)); return TYLO_ERR_CUDA; }
+  return TYLO_OK;
+}
+
+// CTAs per row: a row is dealt over a cluster while rows alone leave SMs without a CTA.
+inline int vocab_parts(int64_t N, int64_t packets, int threads) {
+  int parts = 1;
+  while (parts < 8 && N * parts * 2 <= 2 * sm_count() && packets >= 2LL * parts * threads) parts *= 2;
+  return parts;
+}
 
 inline int32_t check_vocab(const char* who, const void* X, int64_t M, int64_t N, int64_t ldx, float temperature) {
   TYLO_REQUIRE(X, TYLO_ERR_INVALID_ARGUMENT, "%s: X must be non-null", who);
