@@ -57,7 +57,7 @@ __device__ __forceinline__ float teacher_row(const DistillArgs& a, size_t row, f
 }
 
 template <typename T, int THREADS, bool LOSS, bool GRAD>
-__global__ void __launch_bounds__(THREADS) distill_row_kernel(const DistillArgs a, int parts) {
+__global__ void __launch_bounds__(THREADS, (THREADS == 128 ? 4 : 1) * (GRAD ? 3 : 4)) distill_row_kernel(const DistillArgs a, int parts) {
   __shared__ float scratch[100];
   __shared__ float p[TYLO_DISTILL_MAX], xk[TYLO_DISTILL_MAX];
   __shared__ int index[TYLO_DISTILL_MAX];
@@ -67,12 +67,12 @@ __global__ void __launch_bounds__(THREADS) distill_row_kernel(const DistillArgs 
   const VocabPart part(blockIdx.x % parts, parts, r.whole);
   const float it = 1.f / a.temperature, scale = kVocabLog2e / a.temperature;
   VocabStats st;
-  if constexpr (LOSS) st = vocab_thread_stats<T, THREADS, 4, false>(x, r, part, scale);
+  if constexpr (LOSS) st = vocab_thread_stats<T, THREADS, 4, false, GRAD>(x, r, part, scale);
   float mass;
   const float log_norm = teacher_row<THREADS>(a, row, p, index, scratch, mass);
   for (int k = threadIdx.x; k < a.K; k += THREADS) xk[k] = index[k] >= 0 ? Elem<T>::to_f(x[index[k]]) : 0.f;
-  if constexpr (LOSS) vocab_reduce<THREADS>(st, scale, scratch, parts);
-  else st = {a.inMx[row], a.inL[row], 0.f};
+  if constexpr (LOSS) vocab_reduce<THREADS, false>(st, scale, scratch, parts);
+  else st = {a.inMx[row], 0.f, a.inL[row], 0.f};
   const float mo = st.m == -INFINITY ? 0.f : st.m;
   if (LOSS && part.part == 0) {
     const float logL = st.s == 0.f ? 0.f : logf(st.s);
@@ -115,17 +115,16 @@ __global__ void __launch_bounds__(THREADS) distill_row_kernel(const DistillArgs 
 template <typename T, bool LOSS, bool GRAD>
 static int32_t distill_dispatch(const char* who, const DistillArgs& a, int64_t N, cudaStream_t stream) {
   const int64_t packets = a.M / Elem<T>::kVec;
-  constexpr int LONG = GRAD && LOSS ? 1024 : 512;
   if constexpr (!LOSS) {       // nothing to tell one another: plain CTAs, as many per row as fill the GPU several times over
     int parts = 1;
-    while (parts < 64 && N * parts < 16 * sm_count() && packets >= 8LL * parts * LONG) parts *= 2;
+    while (parts < 64 && N * parts < 16 * sm_count() && packets >= 8LL * parts * 512) parts *= 2;
     if (packets <= 1024) distill_row_kernel<T, 128, LOSS, GRAD><<<(unsigned)N, 128, 0, stream>>>(a, 1);
-    else distill_row_kernel<T, LONG, LOSS, GRAD><<<(unsigned)(N * parts), LONG, 0, stream>>>(a, parts);
+    else distill_row_kernel<T, 512, LOSS, GRAD><<<(unsigned)(N * parts), 512, 0, stream>>>(a, parts);
     return check_launch(who);
   } else {
     if (packets <= 1024)
       return launch_vocab(who, distill_row_kernel<T, 128, LOSS, GRAD>, a, N, vocab_parts(N, packets, 128), 128, stream);
-    return launch_vocab(who, distill_row_kernel<T, LONG, LOSS, GRAD>, a, N, vocab_parts(N, packets, LONG), LONG, stream);
+    return launch_vocab(who, distill_row_kernel<T, 512, LOSS, GRAD>, a, N, vocab_parts(N, packets, 512), 512, stream);
   }
 }
 

@@ -45,8 +45,11 @@ struct LogprobGrad {
   }
 };
 
+// CTAs per SM: registers for as many as the loads need to be hidden behind one another
+constexpr int logprob_ctas(int threads, bool entropy, bool top, bool grad) { return (threads == 128 ? 4 : 1) * (top ? 2 : entropy || grad ? 3 : 4); }
+
 template <typename T, int THREADS, bool ENTROPY, bool TOP, bool GRAD>
-__global__ void __launch_bounds__(THREADS) logprob_row_kernel(const LogprobArgs a, int parts) {
+__global__ void __launch_bounds__(THREADS, logprob_ctas(THREADS, ENTROPY, TOP, GRAD)) logprob_row_kernel(const LogprobArgs a, int parts) {
   __shared__ float scratch[100];
   const size_t row = blockIdx.x / parts;
   const T* x = (const T*)a.X + row * a.ldx;
@@ -56,10 +59,10 @@ __global__ void __launch_bounds__(THREADS) logprob_row_kernel(const LogprobArgs 
   const int target = a.targets ? a.targets[row] : -1;
   const bool has = target >= 0 && target < a.M;
   const float xt = has ? Elem<T>::to_f(x[target]) : 0.f;
-  VocabStats st = vocab_thread_stats<T, THREADS, 4, ENTROPY>(x, r, part, scale);
+  VocabStats st = vocab_thread_stats<T, THREADS, 4, ENTROPY, GRAD>(x, r, part, scale);
   uint32_t mine = 0;
   if constexpr (TOP) mine = vocab_mine<T, THREADS>(x, r, part, st);
-  vocab_reduce<THREADS>(st, scale, scratch, parts);
+  vocab_reduce<THREADS, ENTROPY>(st, scale, scratch, parts);
   const float logL = st.s == 0.f ? 0.f : logf(st.s), H = st.s == 0.f ? 0.f : logL - kVocabLn2 * st.a / st.s;
   const float mo = st.m == -INFINITY ? 0.f : st.m;
   if (threadIdx.x == 0 && part.part == 0) {
@@ -84,7 +87,7 @@ __global__ void __launch_bounds__(THREADS) logprob_row_kernel(const LogprobArgs 
 }
 
 template <typename T, int THREADS, bool ENTROPY>
-__global__ void __launch_bounds__(THREADS) logprob_bwd_kernel(const LogprobArgs a, int parts) {
+__global__ void __launch_bounds__(THREADS, 6) logprob_bwd_kernel(const LogprobArgs a, int parts) {
   const size_t row = blockIdx.x / parts;
   const T* x = (const T*)a.X + row * a.ldx;
   const VocabRow<T> r(x, a.M);
@@ -108,20 +111,18 @@ static int32_t logprob_launch(const char* who, const LogprobArgs& a, int64_t N, 
 template <typename T, bool GRAD>
 static int32_t logprob_dispatch(const char* who, const LogprobArgs& a, int64_t N, cudaStream_t stream) {
   const bool entropy = a.Entropy || a.dEntropy;
-  constexpr int LONG = GRAD ? 1024 : 512;
   if (a.M / Elem<T>::kVec <= 1024)
     return entropy ? logprob_launch<T, 128, true, GRAD>(who, a, N, stream) : logprob_launch<T, 128, false, GRAD>(who, a, N, stream);
-  return entropy ? logprob_launch<T, LONG, true, GRAD>(who, a, N, stream) : logprob_launch<T, LONG, false, GRAD>(who, a, N, stream);
+  return entropy ? logprob_launch<T, 512, true, GRAD>(who, a, N, stream) : logprob_launch<T, 512, false, GRAD>(who, a, N, stream);
 }
 
 template <typename T>
 static int32_t logprob_bwd_dispatch(const char* who, const LogprobArgs& a, int64_t N, cudaStream_t stream) {
   constexpr int THREADS = 256;
   const int64_t packets = a.M / Elem<T>::kVec;
-  const int segments = (int)((packets + 4 * THREADS - 1) / (4 * THREADS));
-  const unsigned grid = (unsigned)(N * (segments > 0 ? segments : 1));
-  if (a.dEntropy) logprob_bwd_kernel<T, THREADS, true><<<grid, THREADS, 0, stream>>>(a, segments > 0 ? segments : 1);
-  else logprob_bwd_kernel<T, THREADS, false><<<grid, THREADS, 0, stream>>>(a, segments > 0 ? segments : 1);
+  const int parts = (int)((packets + 4 * THREADS - 1) / (4 * THREADS) + (packets == 0));
+  if (a.dEntropy) logprob_bwd_kernel<T, THREADS, true><<<(unsigned)(N * parts), THREADS, 0, stream>>>(a, parts);
+  else logprob_bwd_kernel<T, THREADS, false><<<(unsigned)(N * parts), THREADS, 0, stream>>>(a, parts);
   return check_launch(who);
 }
 

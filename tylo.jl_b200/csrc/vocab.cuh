@@ -51,50 +51,74 @@ __device__ __forceinline__ uint4 ld_logits(const void* p) {
   return v;
 }
 
-// Running statistics of a row or of a part of it: maximum, sum of exp2((x - m) * scale), sum of the same times its exponent.
+// The same for rows that are read twice: they stay in L2 before what is read or written once.
+__device__ __forceinline__ uint64_t keep_policy() {
+  uint64_t p;
+  asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(p));
+  return p;
+}
+__device__ __forceinline__ uint4 ld_logits(const void* p, uint64_t policy) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.L2::cache_hint.v4.u32 {%0,%1,%2,%3}, [%4], %5;"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p), "l"(policy) : "memory");
+  return v;
+}
+
+// Running statistics of a row or of a part of it: largest logit, the reference that the exponentials are taken against, sum of
+// e = exp2((x - ref) * scale), sum of e times its exponent.  The reference follows the maximum only when that is more than
+// kRefSlack (in units of log 2) above it: sums in floating point are as good, and the branch that rescales them stays rare.
+constexpr float kRefSlack = 8.f;
+
 struct VocabStats {
-  float m, s, a;
-  __device__ __forceinline__ void raise(float to, float scale) {       // to >= m
-    const float d = fmaxf((m - to) * scale, kExpFloor), e = vocab_ex2(d);
+  float m, ref, s, a;
+  __device__ __forceinline__ void refer(float to, float scale) {
+    const float d = fmaxf((ref - to) * scale, kExpFloor), e = vocab_ex2(d);
     a = e * fmaf(d, s, a);
     s *= e;
-    m = to;
-  }
-  __device__ __forceinline__ void join(VocabStats o, float scale) {
-    const float mn = fmaxf(m, o.m);
-    raise(mn, scale);
-    o.raise(mn, scale);
-    s += o.s;
-    a += o.a;
+    ref = to;
   }
 };
 
-__device__ __forceinline__ void vocab_warp_reduce(VocabStats& st, float scale) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-    st.join({__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s, o), __shfl_xor_sync(0xffffffffu, st.a, o)}, scale);
+__device__ __forceinline__ float warp_max(float x) {
+  float y;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));       // a NaN is passed over
+  return y;
 }
 
-// All threads receive the statistics of the CTA, or of the cluster's CTAs that share a row.  `scratch`: 100 floats.  A cluster's CTAs
-// must not leave before all have come back from here (their shared memory is read): see cluster_done.
-template <int THREADS>
+// All threads receive the statistics of the CTA, or of the cluster's CTAs that share a row.  The maximum goes first, so that every
+// thread rescales its sums once.  `scratch`: 100 floats.  A cluster's CTAs must not leave before all have come back from here (their
+// shared memory is read): see cluster_done.
+template <int THREADS, bool ENTROPY>
 __device__ __forceinline__ void vocab_reduce(VocabStats& st, float scale, float* scratch, int parts) {
-  vocab_warp_reduce(st, scale);
+  constexpr int WARPS = THREADS / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (lane == 0) { scratch[warp] = st.m; scratch[32 + warp] = st.s; scratch[64 + warp] = st.a; }
+  float m = warp_max(st.m);
+  if (lane == 0) scratch[warp] = m;
   __syncthreads();
-  const bool live = lane < THREADS / 32;
-  st = {live ? scratch[lane] : -INFINITY, live ? scratch[32 + lane] : 0.f, live ? scratch[64 + lane] : 0.f};
-  vocab_warp_reduce(st, scale);
+  m = warp_max(lane < WARPS ? scratch[lane] : -INFINITY);
+  st.refer(m, scale);
+  float s = warp_reduce(st.s, SumOp()), a = ENTROPY ? warp_reduce(st.a, SumOp()) : 0.f;
+  if (lane == 0) { scratch[32 + warp] = s; scratch[64 + warp] = a; }
+  __syncthreads();
+  s = lane < WARPS ? scratch[32 + lane] : 0.f;
+  a = lane < WARPS ? scratch[64 + lane] : 0.f;
+#pragma unroll
+  for (int o = WARPS / 2; o > 0; o >>= 1) {
+    s += __shfl_xor_sync(0xffffffffu, s, o);
+    if constexpr (ENTROPY) a += __shfl_xor_sync(0xffffffffu, a, o);
+  }
+  st = {m, m, __shfl_sync(0xffffffffu, s, 0), __shfl_sync(0xffffffffu, a, 0)};
   if (parts > 1) {
     cg::cluster_group cluster = cg::this_cluster();
     if (threadIdx.x == 0) { scratch[96] = st.m; scratch[97] = st.s; scratch[98] = st.a; }
     cluster.sync();
     const float* peer = cluster.map_shared_rank(scratch, lane < parts ? lane : 0);
-    st = lane < parts ? VocabStats{peer[96], peer[97], peer[98]} : VocabStats{-INFINITY, 0.f, 0.f};
-    vocab_warp_reduce(st, scale);
+    st = lane < parts ? VocabStats{peer[96], peer[96], peer[97], peer[98]} : VocabStats{-INFINITY, -INFINITY, 0.f, 0.f};
+    st.m = warp_max(st.m);
+    st.refer(st.m, scale);
+    st.s = warp_reduce(st.s, SumOp());
+    if constexpr (ENTROPY) st.a = warp_reduce(st.a, SumOp());
   }
-  __syncthreads();
 }
 
 __device__ __forceinline__ void cluster_done(int parts) {
@@ -142,36 +166,38 @@ template <typename T> __device__ __forceinline__ uint4 no_logits() {
   return make_uint4(w, w, w, w);
 }
 
-// One thread's share of a part: every THREADS-th packet, U at a time with the next U on their way, and a single element.  The
-// exponentials of a step are taken against the thread's own running maximum; sums are kept in two chains (packed fp32 pairs).
-template <typename T, int THREADS, int U, bool ENTROPY>
+// One thread's share of a part: every THREADS-th packet, U at a time, and a single element.  Sums are kept in two chains (packed fp32
+// pairs).  KEEP: the part will be read again.
+template <typename T, int THREADS, int U, bool ENTROPY, bool KEEP>
 __device__ __forceinline__ VocabStats vocab_thread_stats(const T* x, const VocabRow<T>& r, const VocabPart& part, float scale) {
   constexpr int VEC = Elem<T>::kVec;
-  float m = -INFINITY;
+  float m = -INFINITY, ref = -INFINITY;
   float2 s = make_float2(0.f, 0.f), a = s;
   const int one = part.part == 0 ? r.single(threadIdx.x) : -1;
   if (one >= 0) {                                   // (a NaN or +Inf gives a NaN sum here as below)
     const float f = Elem<T>::to_f(x[one]);
-    m = fmaxf(m, f);
-    s.x = vocab_ex2((f - (m == -INFINITY ? 0.f : m)) * scale);
+    m = ref = fmaxf(m, f);
+    s.x = vocab_ex2((f - (ref == -INFINITY ? 0.f : ref)) * scale);
   }
   const T* base = x + r.head;
-  auto load = [&](Pack<T> (&p)[U], int v0) {
+  const uint64_t keep = KEEP ? keep_policy() : 0;
+  for (int v0 = part.lo + threadIdx.x; v0 < part.hi; v0 += U * THREADS) {
+    Pack<T> p[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int v = v0 + u * THREADS;
-      p[u].raw = v < part.hi ? ld_logits(base + (size_t)v * VEC) : no_logits<T>();
+      if (v >= part.hi) p[u].raw = no_logits<T>();
+      else if constexpr (KEEP) p[u].raw = ld_logits(base + (size_t)v * VEC, keep);
+      else p[u].raw = ld_logits(base + (size_t)v * VEC);
     }
-  };
-  auto take = [&](const Pack<T> (&p)[U]) {
-    const float mx = packets_max<T, U>(p);
-    if (mx > m) {
-      const float d = fmaxf((m - mx) * scale, kExpFloor), e = vocab_ex2(d);
+    m = fmaxf(m, packets_max<T, U>(p));
+    if ((m - ref) * scale > kRefSlack) {              // (both -Inf: a NaN, no)
+      const float d = fmaxf((ref - m) * scale, kExpFloor), e = vocab_ex2(d);
       if constexpr (ENTROPY) a = __fmul2_rn(make_float2(e, e), __ffma2_rn(make_float2(d, d), s, a));
       s = __fmul2_rn(make_float2(e, e), s);
-      m = mx;
+      ref = m;
     }
-    const float mo = m == -INFINITY ? 0.f : -m;
+    const float mo = ref == -INFINITY ? 0.f : -ref;
     const float2 nm = make_float2(mo, mo), sc = make_float2(scale, scale);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -185,26 +211,12 @@ __device__ __forceinline__ VocabStats vocab_thread_stats(const T* x, const Vocab
         if constexpr (ENTROPY) a = __ffma2_rn(e, make_float2(fmaxf(y.x, kExpFloor), fmaxf(y.y, kExpFloor)), a);
       }
     }
-  };
-  int v0 = part.lo + threadIdx.x;
-  if (v0 < part.hi) {
-    Pack<T> p[U], q[U];
-    load(p, v0);
-    while (true) {
-      v0 += U * THREADS;
-      if (v0 >= part.hi) { take(p); break; }
-      load(q, v0);
-      take(p);
-      v0 += U * THREADS;
-      if (v0 >= part.hi) { take(q); break; }
-      load(p, v0);
-      take(q);
-    }
   }
-  return {m, s.x + s.y, a.x + a.y};
+  return {m, ref, s.x + s.y, a.x + a.y};
 }
 
-// Second look at a part: f(pair of logits) -> pair of gradients for every element, `at` added to element `hot`.  Rounded once, on the way out.
+// Gradient of a part: f(pair of logits) -> pair of gradients for every element, `at` added to element `hot`.  Rounded once, on the way
+// out.  As the second look at a part it goes backwards: what was read last is the likeliest to be in L2.
 template <typename T, int THREADS, int U, typename F>
 __device__ __forceinline__ void vocab_rewrite(T* dx, const T* x, const VocabRow<T>& r, const VocabPart& part, int hot, float at, F f) {
   constexpr int VEC = Elem<T>::kVec;
@@ -214,12 +226,12 @@ __device__ __forceinline__ void vocab_rewrite(T* dx, const T* x, const VocabRow<
   const int hv = hot >= r.head && hot < r.head + r.whole * VEC ? (hot - r.head) / VEC : -1, hj = (hot - r.head) % VEC;
   x += r.head;
   dx += r.head;
-  auto load = [&](Pack<T> (&p)[U], int v0) {
+  for (int i = (part.hi - part.lo + U * THREADS - 1) / (U * THREADS) - 1; i >= 0; --i) {
+    const int v0 = part.lo + i * (U * THREADS) + threadIdx.x;
+    Pack<T> p[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (v0 + u * THREADS < part.hi) p[u].raw = ld_logits(x + (size_t)(v0 + u * THREADS) * VEC);
-  };
-  auto give = [&](Pack<T> (&p)[U], int v0) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int v = v0 + u * THREADS;
@@ -237,20 +249,6 @@ __device__ __forceinline__ void vocab_rewrite(T* dx, const T* x, const VocabRow<
       p[u].pack(e);
       if (v < part.hi) st_stream(dx + (size_t)v * VEC, p[u].raw);
     }
-  };
-  int v0 = part.lo + threadIdx.x;
-  if (v0 >= part.hi) return;
-  Pack<T> p[U], q[U];
-  load(p, v0);
-  while (true) {
-    const int v1 = v0 + U * THREADS;
-    if (v1 >= part.hi) { give(p, v0); break; }
-    load(q, v1);
-    give(p, v0);
-    v0 = v1 + U * THREADS;
-    if (v0 >= part.hi) { give(q, v1); break; }
-    load(p, v0);
-    give(q, v1);
   }
 }
 
@@ -283,7 +281,8 @@ template <int THREADS> struct TopScratch {
   uint64_t few[TYLO_TOP_MAX + kTopSlack];
   uint64_t sorted[TYLO_TOP_MAX];
   uint32_t warp[64];
-  int n, m;
+  uint16_t who[THREADS];
+  int n, m, w;
 };
 
 template <int THREADS> struct BlockCount {
@@ -301,43 +300,15 @@ template <int THREADS> struct BlockCount {
   }
 };
 
-// Applies f(value, index) to the elements of this thread's share, in the share's order; `some(packet's values)` may skip a packet.
-template <typename T, int THREADS, typename S, typename F>
-__device__ __forceinline__ void vocab_share(const T* x, const VocabRow<T>& r, const VocabPart& part, S some, F f) {
-  constexpr int VEC = Elem<T>::kVec, U = 4;
-  const int one = part.part == 0 ? r.single(threadIdx.x) : -1;
-  if (one >= 0) f(Elem<T>::to_f(x[one]), one);
-  for (int v0 = part.lo + threadIdx.x; v0 < part.hi; v0 += U * THREADS) {
-    Pack<T> p[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (v0 + u * THREADS < part.hi) p[u].raw = ld_logits(x + r.index(v0 + u * THREADS));
-#pragma unroll 1
-    for (int u = 0; u < U; ++u) {
-      const int v = v0 + u * THREADS;
-      Pack<T> q = p[0];
-#pragma unroll
-      for (int w = 1; w < U; ++w)
-        if (w == u) q = p[w];
-      if (v >= part.hi) break;
-      float e[VEC];
-      q.unpack(e);
-      if (!some(e)) continue;
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) f(e[j], r.index(v) + j);
-    }
-  }
-}
-
 // Puts the min(K, elements of the part) largest elements of the part into sc.sorted, in falling order, and returns how many.
 // `mine`: this thread's largest element as a key, 0 without elements.
 template <typename T, int THREADS>
-__device__ int vocab_top(const T* x, const VocabRow<T>& r, const VocabPart& part, int K, uint32_t mine, TopScratch<THREADS>& sc) {
+__device__ __noinline__ int vocab_top(const T* x, const VocabRow<T> r, const VocabPart part, int K, uint32_t mine, TopScratch<THREADS>& sc) {
   constexpr int VEC = Elem<T>::kVec, kTopSlots = TopScratch<THREADS>::kSlots;
   const int elements = (part.hi - part.lo) * VEC + (part.part == 0 ? r.head + r.tail : 0);
   K = min(K, elements);
   BlockCount<THREADS> count{sc.warp, 0};
-  if (threadIdx.x == 0) { sc.n = 0; sc.m = 0; }
+  if (threadIdx.x == 0) { sc.n = 0; sc.m = 0; sc.w = 0; }
   const int lane = threadIdx.x & 31;
   // largest and smallest key among the threads that have one
   uint32_t hi = __reduce_max_sync(0xffffffffu, mine), lo = __reduce_min_sync(0xffffffffu, mine ? mine : 0xffffffffu);
@@ -360,33 +331,75 @@ __device__ int vocab_top(const T* x, const VocabRow<T>& r, const VocabPart& part
     }
     t = lo;
   }
-  // elements above or at a bound; what does not fit is counted all the same
+  // Hands the elements of the threads whose maximum reaches `from` to f(values, number of values, first index) by the packet.  The
+  // packets of those threads are dealt over the whole CTA; f returns false when it has seen enough.
+  auto visit = [&](uint32_t from, auto f) {
+    if (mine >= from) sc.who[atomicAdd(&sc.w, 1)] = threadIdx.x;
+    __syncthreads();
+    const int w = sc.w, per = (part.hi - part.lo + THREADS - 1) / THREADS, all = w * per;
+    constexpr int U = 4;
+    bool more = true;
+    const int one = part.part == 0 && mine >= from ? r.single(threadIdx.x) : -1;
+    if (one >= 0) {
+      float e[VEC];
+      e[0] = Elem<T>::to_f(x[one]);
+      more = f(e, 1, one);
+    }
+    for (int i0 = threadIdx.x; i0 < all && more; i0 += U * THREADS) {
+      Pack<T> p[U];
+      int v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * THREADS;
+        v[u] = i < all ? part.lo + sc.who[i % w] + i / w * THREADS : part.hi;
+        if (v[u] < part.hi) p[u].raw = ld_logits(x + r.index(v[u]));
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (v[u] < part.hi && more) {
+          float e[VEC];
+          p[u].unpack(e);
+          more = f(e, VEC, r.index(v[u]));
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) sc.w = 0;
+    __syncthreads();
+  };
+  // elements above or at a bound into sc.keys; more than kTopSlots: at least that many
   auto collect = [&](uint32_t from) {
     const float low = from <= 1 ? -INFINITY : vocab_unkey(from);
-    if (mine >= from)
-      vocab_share<T, THREADS>(x, r, part, [&](const float (&e)[VEC]) {
-        bool any = false;
+    visit(from, [&](const float (&e)[VEC], int n, int first) {
+      uint32_t hit = 0;
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) any |= !(e[j] < low);
-        return any;
-      }, [&](float e, int j) {
-        if (vocab_key(e) >= from) {
-          const int at = atomicAdd(&sc.n, 1);
-          if (at < kTopSlots) sc.keys[at] = vocab_key(e, j);
+      for (int j = 0; j < VEC; ++j) hit |= (uint32_t)(j < n && !(e[j] < low)) << j;
+      if (!hit) return true;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j)
+        if ((hit >> j & 1) && vocab_key(e[j]) < from) hit &= ~(1u << j);           // NaN, and bounds without a value of their own
+      const int at = atomicAdd(&sc.n, __popc(hit));
+      int k = at;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j)
+        if (hit >> j & 1) {
+          if (k < kTopSlots) sc.keys[k] = vocab_key(e[j], first + j);
+          ++k;
         }
-      });
-    __syncthreads();
-    const int n = sc.n;
-    __syncthreads();
-    return n;
+      return at < kTopSlots;
+    });
+    return sc.n;
   };
   auto at_least = [&](uint32_t from) {
     int c = 0;
-    if (mine >= from)
-      vocab_share<T, THREADS>(x, r, part, [](const float (&)[VEC]) { return true; }, [&](float e, int) { c += vocab_key(e) >= from; });
+    visit(from, [&](const float (&e)[VEC], int n, int) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) c += j < n && vocab_key(e[j]) >= from;
+      return true;
+    });
     return count(c);
   };
   auto clear = [&]() {
+    __syncthreads();
     if (threadIdx.x == 0) sc.n = 0;
     __syncthreads();
   };
@@ -531,9 +544,12 @@ __device__ __forceinline__ void vocab_ranked(TopScratch<THREADS>& sc, int n, int
 template <typename T, int THREADS>
 __device__ __forceinline__ uint32_t vocab_mine(const T* x, const VocabRow<T>& r, const VocabPart& part, const VocabStats& st) {
   uint32_t k = 0;
+  const int one = part.part == 0 ? r.single(threadIdx.x) : -1;
   if (st.s != st.s) {
-    vocab_share<T, THREADS>(x, r, part, [](const float (&)[Elem<T>::kVec]) { return true; }, [&](float e, int) { k = max(k, vocab_key(e)); });
-  } else if (part.lo + (int)threadIdx.x < part.hi || (part.part == 0 && r.single(threadIdx.x) >= 0)) {
+    if (one >= 0) k = vocab_key(Elem<T>::to_f(x[one]));
+    for (int v = part.lo + threadIdx.x; v < part.hi; v += THREADS)
+      for (int j = 0; j < Elem<T>::kVec; ++j) k = max(k, vocab_key(Elem<T>::to_f(x[r.index(v) + j])));
+  } else if (part.lo + (int)threadIdx.x < part.hi || one >= 0) {
     k = vocab_key(st.m);
   }
   return k;
