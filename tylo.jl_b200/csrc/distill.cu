@@ -89,25 +89,26 @@ __global__ void __launch_bounds__(THREADS, (THREADS == 128 ? 4 : 1) * (GRAD ? 3 
   if constexpr (GRAD) {
     T* dx = (T*)a.dX + row * a.ldx;
     const float w = a.dLoss[row] * it;
-    const bool none = w == 0.f || mass == 0.f || st.s == 0.f;
-    const float c = none ? 0.f : w * mass / st.s;
-    auto grad = [&](float2 f) {
-      const float2 y = __fmul2_rn(__fadd2_rn(f, make_float2(-mo, -mo)), make_float2(scale, scale));
-      const float2 d = __fmul2_rn(make_float2(vocab_ex2(y.x), vocab_ex2(y.y)), make_float2(c, c));
-      return none ? make_float2(0.f, 0.f) : d;
-    };
-    if (!LOSS) __syncthreads();             // xk is read before any gradient is written: dX may be X
-    vocab_rewrite<T, THREADS, 4>(dx, x, r, part, -1, 0.f, grad);
-    __syncthreads();
-    // the teacher's entries in this part: every copy of an index sums all its copies in the same order and stores the same value
-    if (!none)
+    if (w == 0.f || mass == 0.f || st.s == 0.f) {       // no weight, no teacher or no probability anywhere
+      vocab_zero<T, THREADS>(dx, r, part);
+    } else {
+      const float2 m2 = make_float2(-mo, -mo), sc = make_float2(scale, scale), c = make_float2(w * mass / st.s, w * mass / st.s);
+      auto grad = [&](float2 f) {
+        const float2 y = __fmul2_rn(__fadd2_rn(f, m2), sc);
+        return __fmul2_rn(make_float2(vocab_ex2(y.x), vocab_ex2(y.y)), c);
+      };
+      if (!LOSS) __syncthreads();             // xk is read before any gradient is written: dX may be X
+      vocab_rewrite<T, THREADS, 4>(dx, x, r, part, grad);
+      __syncthreads();
+      // the teacher's entries in this part: every copy of an index sums all its copies in the same order and stores the same value
       for (int k = threadIdx.x; k < a.K; k += THREADS) {
         const int j = index[k];
-        if (j < 0 || !part.holds(r, j)) continue;
+        if (j < 0 || part.template owner<THREADS>(r, j) < 0) continue;
         float sum = 0.f;
         for (int i = 0; i < a.K; ++i) sum += index[i] == j ? p[i] : 0.f;
         dx[j] = Elem<T>::from_f(grad(make_float2(xk[k], 0.f)).x - w * sum);
       }
+    }
   }
   if constexpr (LOSS) cluster_done(parts);
 }

@@ -19,31 +19,39 @@ struct LogprobArgs {
   float temperature;
 };
 
-// What a row's gradient needs: dX_j = e_j (A y_j + B) with e_j = exp2(y_j), y_j in units of log 2, and `at` at the target.
-struct LogprobGrad {
-  float mo, scale, A, B, at;
-  bool none;
+// A row's gradient: dX_j = e_j (A y_j + B) with e_j = exp2(y_j), y_j in units of log 2, and `at` added at the target.
+template <bool ENTROPY> struct LogprobGrad {
+  float2 mo, scale, A, B;
+  float at;
   __device__ __forceinline__ LogprobGrad(float mx, float L, float g, float h, float H, float temperature) {
-    const float it = 1.f / temperature, inv = 1.f / L;
-    none = (g == 0.f && h == 0.f) || L == 0.f;
-    mo = mx == -INFINITY ? 0.f : mx;
-    scale = kVocabLog2e * it;
+    const float it = 1.f / temperature, c = it / L, m = mx == -INFINITY ? 0.f : -mx, k = kVocabLog2e * it;
     // -p (g + h (log p + H)) / t with log p = ln 2 (y - log2 L)
-    A = -h * kVocabLn2 * it * inv;
-    B = -(g + (h == 0.f ? 0.f : h * (H - logf(L)))) * it * inv;
-    at = none ? 0.f : g * it;
+    const float a = -h * kVocabLn2 * c, b = -(ENTROPY ? g + h * (H - logf(L)) : g) * c;
+    mo = make_float2(m, m); scale = make_float2(k, k); A = make_float2(a, a); B = make_float2(b, b);
+    at = g * it;
   }
-  template <bool ENTROPY> __device__ __forceinline__ float2 operator()(float2 x) const {
-    const float2 y = __fmul2_rn(__fadd2_rn(x, make_float2(-mo, -mo)), make_float2(scale, scale));
+  __device__ __forceinline__ float2 operator()(float2 x) const {
+    const float2 y = __fmul2_rn(__fadd2_rn(x, mo), scale);
     const float2 e = make_float2(vocab_ex2(y.x), vocab_ex2(y.y));
-    float2 d;
-    if constexpr (ENTROPY)
-      d = __fmul2_rn(e, __ffma2_rn(make_float2(A, A), make_float2(fmaxf(y.x, kExpFloor), fmaxf(y.y, kExpFloor)), make_float2(B, B)));
-    else
-      d = __fmul2_rn(e, make_float2(B, B));
-    return none ? make_float2(0.f, 0.f) : d;
+    if constexpr (ENTROPY) return __fmul2_rn(e, __ffma2_rn(A, make_float2(fmaxf(y.x, kExpFloor), fmaxf(y.y, kExpFloor)), B));
+    else return __fmul2_rn(e, B);
   }
 };
+
+// The gradient of a part.  `xt`: the target's logit, read before anything is written (dX may be X); target < 0: none.  A row without
+// weights or without any probability gets zeros.
+template <typename T, int THREADS, bool ENTROPY>
+__device__ __forceinline__ void logprob_part_grad(const LogprobArgs& a, size_t row, const T* x, const VocabRow<T>& r, const VocabPart& part,
+                                                  int target, float xt, float mx, float L, float g, float h, float H) {
+  T* dx = (T*)a.dX + row * a.ldx;
+  if ((g == 0.f && h == 0.f) || L == 0.f) {
+    vocab_zero<T, THREADS>(dx, r, part);
+    return;
+  }
+  const LogprobGrad<ENTROPY> d(mx, L, g, h, H, a.temperature);
+  vocab_rewrite<T, THREADS, 4>(dx, x, r, part, d);
+  if (target >= 0 && part.template owner<THREADS>(r, target) == (int)threadIdx.x) dx[target] = Elem<T>::from_f(d(make_float2(xt, 0.f)).x + d.at);
+}
 
 // CTAs per SM: registers for as many as the loads need to be hidden behind one another
 constexpr int logprob_ctas(int threads, bool entropy, bool top, bool grad) { return (threads == 128 ? 4 : 1) * (top ? 2 : entropy || grad ? 3 : 4); }
@@ -78,11 +86,9 @@ __global__ void __launch_bounds__(THREADS, logprob_ctas(THREADS, ENTROPY, TOP, G
       a.TopIndex[row * a.top + rank] = vocab_key_index(key);
     });
   }
-  if constexpr (GRAD) {
-    const LogprobGrad d(st.m, st.s, has ? a.dLogp[row] : 0.f, a.dEntropy ? a.dEntropy[row] : 0.f, H, a.temperature);
-    vocab_rewrite<T, THREADS, 4>((T*)a.dX + row * a.ldx, x, r, part, has ? target : -1, d.at,
-                                 [&](float2 f) { return d.template operator()<ENTROPY>(f); });
-  }
+  if constexpr (GRAD)
+    logprob_part_grad<T, THREADS, ENTROPY>(a, row, x, r, part, has ? target : -1, xt, st.m, st.s, has ? a.dLogp[row] : 0.f,
+                                           ENTROPY && a.dEntropy ? a.dEntropy[row] : 0.f, H);
   cluster_done(parts);
 }
 
@@ -94,10 +100,10 @@ __global__ void __launch_bounds__(THREADS, 6) logprob_bwd_kernel(const LogprobAr
   const VocabPart part(blockIdx.x % parts, parts, r.whole);
   const int target = a.targets ? a.targets[row] : -1;
   const bool has = target >= 0 && target < a.M;
-  const LogprobGrad d(a.inMx[row], a.inL[row], has ? a.dLogp[row] : 0.f, ENTROPY ? a.dEntropy[row] : 0.f, ENTROPY ? a.inEntropy[row] : 0.f,
-                      a.temperature);
-  vocab_rewrite<T, THREADS, 4>((T*)a.dX + row * a.ldx, x, r, part, has ? target : -1, d.at,
-                               [&](float2 f) { return d.template operator()<ENTROPY>(f); });
+  const float xt = has ? Elem<T>::to_f(x[target]) : 0.f;
+  // (in place: the thread that uses xt is the one that writes its packet, later)
+  logprob_part_grad<T, THREADS, ENTROPY>(a, row, x, r, part, has ? target : -1, xt, a.inMx[row], a.inL[row], has ? a.dLogp[row] : 0.f,
+                                         ENTROPY ? a.dEntropy[row] : 0.f, ENTROPY ? a.inEntropy[row] : 0.f);
 }
 
 template <typename T, int THREADS, bool ENTROPY, bool GRAD>
@@ -120,7 +126,7 @@ template <typename T>
 static int32_t logprob_bwd_dispatch(const char* who, const LogprobArgs& a, int64_t N, cudaStream_t stream) {
   constexpr int THREADS = 256;
   const int64_t packets = a.M / Elem<T>::kVec;
-  const int parts = (int)((packets + 4 * THREADS - 1) / (4 * THREADS) + (packets == 0));
+  const int parts = (int)((packets + 8 * THREADS - 1) / (8 * THREADS) + (packets == 0));
   if (a.dEntropy) logprob_bwd_kernel<T, THREADS, true><<<(unsigned)(N * parts), THREADS, 0, stream>>>(a, parts);
   else logprob_bwd_kernel<T, THREADS, false><<<(unsigned)(N * parts), THREADS, 0, stream>>>(a, parts);
   return check_launch(who);

@@ -133,10 +133,13 @@ struct VocabPart {
     lo = min(part * per, whole);
     hi = min(lo + per, whole);
   }
-  template <typename R> __device__ __forceinline__ bool holds(const R& r, int index) const {
+  // Which thread of this part's CTA works on element `index`, -1: none.
+  template <int THREADS, typename R> __device__ __forceinline__ int owner(const R& r, int index) const {
     const int e = index - r.head;
-    if (e < 0 || e >= r.whole * R::kVec) return part == 0;
-    return e / R::kVec >= lo && e / R::kVec < hi;
+    if (e < 0) return part == 0 ? index : -1;
+    const int v = e / R::kVec;
+    if (v >= r.whole) return part == 0 ? r.head + index - (r.M - r.tail) : -1;
+    return v >= lo && v < hi ? (v - lo) % THREADS : -1;
   }
 };
 
@@ -179,17 +182,8 @@ __device__ __forceinline__ VocabStats vocab_thread_stats(const T* x, const Vocab
     m = ref = fmaxf(m, f);
     s.x = vocab_ex2((f - (ref == -INFINITY ? 0.f : ref)) * scale);
   }
-  const T* base = x + r.head;
-  const uint64_t keep = KEEP ? keep_policy() : 0;
-  for (int v0 = part.lo + threadIdx.x; v0 < part.hi; v0 += U * THREADS) {
-    Pack<T> p[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int v = v0 + u * THREADS;
-      if (v >= part.hi) p[u].raw = no_logits<T>();
-      else if constexpr (KEEP) p[u].raw = ld_logits(base + (size_t)v * VEC, keep);
-      else p[u].raw = ld_logits(base + (size_t)v * VEC);
-    }
+  const float2 sc = make_float2(scale, scale);
+  auto take = [&](const Pack<T> (&p)[U]) {
     m = fmaxf(m, packets_max<T, U>(p));
     if ((m - ref) * scale > kRefSlack) {              // (both -Inf: a NaN, no)
       const float d = fmaxf((ref - m) * scale, kExpFloor), e = vocab_ex2(d);
@@ -198,7 +192,7 @@ __device__ __forceinline__ VocabStats vocab_thread_stats(const T* x, const Vocab
       ref = m;
     }
     const float mo = ref == -INFINITY ? 0.f : -ref;
-    const float2 nm = make_float2(mo, mo), sc = make_float2(scale, scale);
+    const float2 nm = make_float2(mo, mo);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       float f[VEC];
@@ -211,45 +205,78 @@ __device__ __forceinline__ VocabStats vocab_thread_stats(const T* x, const Vocab
         if constexpr (ENTROPY) a = __ffma2_rn(e, make_float2(fmaxf(y.x, kExpFloor), fmaxf(y.y, kExpFloor)), a);
       }
     }
+  };
+  const uint64_t keep = KEEP ? keep_policy() : 0;
+  const T* q = x + r.index(part.lo + threadIdx.x);
+  auto load = [&](Pack<T>& p, int u) {
+    if constexpr (KEEP) p.raw = ld_logits(q + u * (THREADS * VEC), keep);
+    else p.raw = ld_logits(q + u * (THREADS * VEC));
+  };
+  int left = part.hi - part.lo - (int)threadIdx.x;    // packets from this thread's next one to the part's end
+  Pack<T> p[U];
+  for (; left > (U - 1) * THREADS; left -= U * THREADS, q += U * THREADS * VEC) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) load(p[u], u);
+    take(p);
+  }
+  if (left > 0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (left > u * THREADS) load(p[u], u);
+      else p[u].raw = no_logits<T>();
+    }
+    take(p);
   }
   return {m, ref, s.x + s.y, a.x + a.y};
 }
 
-// Gradient of a part: f(pair of logits) -> pair of gradients for every element, `at` added to element `hot`.  Rounded once, on the way
-// out.  As the second look at a part it goes backwards: what was read last is the likeliest to be in L2.
+// Gradient of a part: f(pair of logits) -> pair of gradients for every element, rounded once, on the way out.  As the second look at a
+// part it goes backwards: what was read last is the likeliest to be in L2.
 template <typename T, int THREADS, int U, typename F>
-__device__ __forceinline__ void vocab_rewrite(T* dx, const T* x, const VocabRow<T>& r, const VocabPart& part, int hot, float at, F f) {
+__device__ __forceinline__ void vocab_rewrite(T* dx, const T* x, const VocabRow<T>& r, const VocabPart& part, F f) {
   constexpr int VEC = Elem<T>::kVec;
   const int one = part.part == 0 ? r.single(threadIdx.x) : -1;
-  if (one >= 0) dx[one] = Elem<T>::from_f(f(make_float2(Elem<T>::to_f(x[one]), 0.f)).x + (one == hot ? at : 0.f));
-  // packet and place of `hot`; -1 where it is a single element or not there
-  const int hv = hot >= r.head && hot < r.head + r.whole * VEC ? (hot - r.head) / VEC : -1, hj = (hot - r.head) % VEC;
-  x += r.head;
-  dx += r.head;
-  for (int i = (part.hi - part.lo + U * THREADS - 1) / (U * THREADS) - 1; i >= 0; --i) {
-    const int v0 = part.lo + i * (U * THREADS) + threadIdx.x;
+  if (one >= 0) dx[one] = Elem<T>::from_f(f(make_float2(Elem<T>::to_f(x[one]), 0.f)).x);
+  auto give = [&](Pack<T>& p, T* to) {
+    float e[VEC];
+    p.unpack(e);
+#pragma unroll
+    for (int j = 0; j < VEC; j += 2) {
+      const float2 d = f(make_float2(e[j], e[j + 1]));
+      e[j] = d.x; e[j + 1] = d.y;
+    }
+    p.pack(e);
+    st_stream(to, p.raw);
+  };
+  const int n = part.hi - part.lo, steps = n / (U * THREADS);
+  const int first = r.index(part.lo + threadIdx.x);
+  {
+    const int i = first + steps * (U * THREADS * VEC), left = n - steps * (U * THREADS) - (int)threadIdx.x;
     Pack<T> p[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (v0 + u * THREADS < part.hi) p[u].raw = ld_logits(x + (size_t)(v0 + u * THREADS) * VEC);
+      if (left > u * THREADS) p[u].raw = ld_logits(x + i + u * (THREADS * VEC));
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int v = v0 + u * THREADS;
-      float e[VEC];
-      p[u].unpack(e);
-#pragma unroll
-      for (int j = 0; j < VEC; j += 2) {
-        const float2 d = f(make_float2(e[j], e[j + 1]));
-        e[j] = d.x; e[j + 1] = d.y;
-      }
-      if (v == hv) {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) e[j] += j == hj ? at : 0.f;
-      }
-      p[u].pack(e);
-      if (v < part.hi) st_stream(dx + (size_t)v * VEC, p[u].raw);
-    }
+    for (int u = 0; u < U; ++u)
+      if (left > u * THREADS) give(p[u], dx + i + u * (THREADS * VEC));
   }
+  for (int k = steps - 1; k >= 0; --k) {
+    const T* q = x + first + k * (U * THREADS * VEC);
+    T* to = dx + first + k * (U * THREADS * VEC);
+    Pack<T> p[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) p[u].raw = ld_logits(q + u * (THREADS * VEC));
+#pragma unroll
+    for (int u = 0; u < U; ++u) give(p[u], to + u * (THREADS * VEC));
+  }
+}
+
+// A gradient of zeros.
+template <typename T, int THREADS>
+__device__ __forceinline__ void vocab_zero(T* dx, const VocabRow<T>& r, const VocabPart& part) {
+  const int one = part.part == 0 ? r.single(threadIdx.x) : -1;
+  if (one >= 0) dx[one] = Elem<T>::from_f(0.f);
+  for (int v = part.lo + threadIdx.x; v < part.hi; v += THREADS) st_stream(dx + r.index(v), make_uint4(0, 0, 0, 0));
 }
 
 // Order of the alternatives as whole numbers: larger logits first, the lower index first among equals, a NaN above everything.
