@@ -23,6 +23,9 @@ struct DistillArgs {
   float temperature, teacher_temperature;
 };
 
+// Places for K entries in each of the three arrays, so that what follows them is 16-byte aligned.
+__host__ __device__ constexpr int entry_slots(int K) { return (K + 3) / 4 * 4; }
+
 // The teacher's probabilities of a row into shared memory (-1 as the index of an entry that is left out); returns the normaliser's
 // logarithm, so that log p_k = v_k / u - the result, and P through `mass`.
 template <int THREADS>
@@ -56,18 +59,24 @@ __device__ __forceinline__ float teacher_row(const DistillArgs& a, size_t row, f
   return log_norm;
 }
 
-template <typename T, int THREADS, bool LOSS, bool GRAD>
-__global__ void __launch_bounds__(THREADS, (THREADS == 128 ? 4 : 1) * (GRAD ? 3 : 4)) distill_row_kernel(const DistillArgs a, int parts) {
+// GROUPS > 0: the part waits in shared memory for the second look.  Dynamic shared memory: the teacher's entries, then the part.
+template <typename T, int THREADS, int U, int GROUPS, bool LOSS, bool GRAD>
+__global__ void __launch_bounds__(THREADS, THREADS == 128 ? 8 : THREADS == 256 ? 5 : GROUPS ? 2 : GRAD ? 3 : 4)
+distill_row_kernel(const DistillArgs a, int parts) {
   __shared__ float scratch[100];
-  __shared__ float p[TYLO_DISTILL_MAX], xk[TYLO_DISTILL_MAX];
-  __shared__ int index[TYLO_DISTILL_MAX];
+  extern __shared__ uint4 dynamic[];
+  const int slots = entry_slots(a.K);
+  float *p = reinterpret_cast<float*>(dynamic), *xk = p + slots;
+  int* index = reinterpret_cast<int*>(xk + slots);
+  uint4* kept = reinterpret_cast<uint4*>(index + slots);
   const size_t row = blockIdx.x / parts;
   const T* x = (const T*)a.X + row * a.ldx;
   const VocabRow<T> r(x, a.M);
   const VocabPart part(blockIdx.x % parts, parts, r.whole);
   const float it = 1.f / a.temperature, scale = kVocabLog2e / a.temperature;
   VocabStats st;
-  if constexpr (LOSS) st = vocab_thread_stats<T, THREADS, 4, false, GRAD>(x, r, part, scale);
+  if constexpr (GROUPS > 0) st = vocab_resident_stats<T, THREADS, U, GROUPS, false>(kept, x, r, part, scale);
+  else if constexpr (LOSS) st = vocab_thread_stats<T, THREADS, U, false, GRAD>(x, r, part, scale);
   float mass;
   const float log_norm = teacher_row<THREADS>(a, row, p, index, scratch, mass);
   for (int k = threadIdx.x; k < a.K; k += THREADS) xk[k] = index[k] >= 0 ? Elem<T>::to_f(x[index[k]]) : 0.f;
@@ -98,7 +107,8 @@ __global__ void __launch_bounds__(THREADS, (THREADS == 128 ? 4 : 1) * (GRAD ? 3 
         return __fmul2_rn(make_float2(vocab_ex2(y.x), vocab_ex2(y.y)), c);
       };
       if (!LOSS) __syncthreads();             // xk is read before any gradient is written: dX may be X
-      vocab_rewrite<T, THREADS, 4>(dx, x, r, part, grad);
+      if constexpr (GROUPS > 0) vocab_resident_rewrite<T, THREADS, U>(dx, kept, x, r, part, grad);
+      else vocab_rewrite<T, THREADS, U>(dx, x, r, part, grad);
       __syncthreads();
       // the teacher's entries in this part: every copy of an index sums all its copies in the same order and stores the same value
       for (int k = threadIdx.x; k < a.K; k += THREADS) {
@@ -116,16 +126,25 @@ __global__ void __launch_bounds__(THREADS, (THREADS == 128 ? 4 : 1) * (GRAD ? 3 
 template <typename T, bool LOSS, bool GRAD>
 static int32_t distill_dispatch(const char* who, const DistillArgs& a, int64_t N, cudaStream_t stream) {
   const int64_t packets = a.M / Elem<T>::kVec;
+  const int entries = 12 * entry_slots(a.K);
   if constexpr (!LOSS) {       // nothing to tell one another: plain CTAs, as many per row as fill the GPU several times over
     int parts = 1;
     while (parts < 64 && N * parts < 16 * sm_count() && packets >= 8LL * parts * 512) parts *= 2;
-    if (packets <= 1024) distill_row_kernel<T, 128, LOSS, GRAD><<<(unsigned)N, 128, 0, stream>>>(a, 1);
-    else distill_row_kernel<T, 512, LOSS, GRAD><<<(unsigned)(N * parts), 512, 0, stream>>>(a, parts);
+    if (packets <= 1024) distill_row_kernel<T, 128, 4, 0, LOSS, GRAD><<<(unsigned)N, 128, entries, stream>>>(a, 1);
+    else distill_row_kernel<T, 512, 4, 0, LOSS, GRAD><<<(unsigned)(N * parts), 512, entries, stream>>>(a, parts);
     return check_launch(who);
   } else {
-    if (packets <= 1024)
-      return launch_vocab(who, distill_row_kernel<T, 128, LOSS, GRAD>, a, N, vocab_parts(N, packets, 128), 128, stream);
-    return launch_vocab(who, distill_row_kernel<T, 512, LOSS, GRAD>, a, N, vocab_parts(N, packets, 512), 512, stream);
+    const int parts = vocab_parts(N, packets);
+    if constexpr (!GRAD) {
+      if (packets <= 1024) return launch_vocab(who, distill_row_kernel<T, 128, 4, 0, LOSS, GRAD>, a, N, parts, 128, stream, entries);
+      return launch_vocab(who, distill_row_kernel<T, 512, 4, 0, LOSS, GRAD>, a, N, parts, 512, stream, entries);
+    } else {
+      const int64_t per = (packets + parts - 1) / parts;
+#define TYLO_BOTH(THREADS, U, GROUPS) \
+  launch_vocab(who, distill_row_kernel<T, THREADS, U, GROUPS, LOSS, GRAD>, a, N, parts, THREADS, stream, entries + (GROUPS ? (int)per * 16 : 0))
+      TYLO_VOCAB_RESIDENT(TYLO_BOTH);
+#undef TYLO_BOTH
+    }
   }
 }
 

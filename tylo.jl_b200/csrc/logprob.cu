@@ -19,6 +19,13 @@ struct LogprobArgs {
   float temperature;
 };
 
+__device__ __forceinline__ float vocab_logp(float x, const VocabStats& st, float temperature) {
+  return (x - (st.m == -INFINITY ? 0.f : st.m)) / temperature - (st.s == 0.f ? 0.f : logf(st.s));
+}
+__device__ __forceinline__ float vocab_entropy(const VocabStats& st) {
+  return st.s == 0.f ? 0.f : logf(st.s) - kVocabLn2 * st.a / st.s;
+}
+
 // A row's gradient: dX_j = e_j (A y_j + B) with e_j = exp2(y_j), y_j in units of log 2, and `at` added at the target.
 template <bool ENTROPY> struct LogprobGrad {
   float2 mo, scale, A, B;
@@ -38,26 +45,63 @@ template <bool ENTROPY> struct LogprobGrad {
   }
 };
 
-// The gradient of a part.  `xt`: the target's logit, read before anything is written (dX may be X); target < 0: none.  A row without
-// weights or without any probability gets zeros.
-template <typename T, int THREADS, bool ENTROPY>
-__device__ __forceinline__ void logprob_part_grad(const LogprobArgs& a, size_t row, const T* x, const VocabRow<T>& r, const VocabPart& part,
-                                                  int target, float xt, float mx, float L, float g, float h, float H) {
+// The gradient of a part, which waits in `kept` or is read (again).  `xt`: the target's logit, read before anything is written (dX may
+// be X); target < 0: none.  A row without weights or without any probability gets zeros.
+template <typename T, int THREADS, int U, bool ENTROPY>
+__device__ __forceinline__ void logprob_part_grad(const LogprobArgs& a, size_t row, const T* x, const uint4* kept, const VocabRow<T>& r,
+                                                  const VocabPart& part, int target, float xt, float mx, float L, float g, float h, float H) {
   T* dx = (T*)a.dX + row * a.ldx;
   if ((g == 0.f && h == 0.f) || L == 0.f) {
     vocab_zero<T, THREADS>(dx, r, part);
     return;
   }
   const LogprobGrad<ENTROPY> d(mx, L, g, h, H, a.temperature);
-  vocab_rewrite<T, THREADS, 4>(dx, x, r, part, d);
+  if (kept) vocab_resident_rewrite<T, THREADS, U>(dx, kept, x, r, part, d);
+  else vocab_rewrite<T, THREADS, U>(dx, x, r, part, d);
   if (target >= 0 && part.template owner<THREADS>(r, target) == (int)threadIdx.x) dx[target] = Elem<T>::from_f(d(make_float2(xt, 0.f)).x + d.at);
 }
 
-// CTAs per SM: registers for as many as the loads need to be hidden behind one another
-constexpr int logprob_ctas(int threads, bool entropy, bool top, bool grad) { return (threads == 128 ? 4 : 1) * (top ? 2 : entropy || grad ? 3 : 4); }
+// CTAs per SM: registers for as many as the loads need to be hidden behind one another, or as shared memory holds
+constexpr int logprob_ctas(int threads, bool entropy, bool top) { return (threads == 128 ? 4 : 1) * (top ? 2 : entropy ? 3 : 4); }
 
-template <typename T, int THREADS, bool ENTROPY, bool TOP, bool GRAD>
-__global__ void __launch_bounds__(THREADS, logprob_ctas(THREADS, ENTROPY, TOP, GRAD)) logprob_row_kernel(const LogprobArgs a, int parts) {
+template <typename T, int THREADS, bool ENTROPY, bool TOP>
+__global__ void __launch_bounds__(THREADS, logprob_ctas(THREADS, ENTROPY, TOP)) logprob_fwd_kernel(const LogprobArgs a, int parts) {
+  __shared__ float scratch[100];
+  const size_t row = blockIdx.x / parts;
+  const T* x = (const T*)a.X + row * a.ldx;
+  const VocabRow<T> r(x, a.M);
+  const VocabPart part(blockIdx.x % parts, parts, r.whole);
+  const float scale = kVocabLog2e / a.temperature;
+  const bool lead = threadIdx.x == 0 && part.part == 0;
+  const int target = lead && a.Logp ? a.targets[row] : -1;
+  const bool has = target >= 0 && target < a.M;
+  const float xt = has ? Elem<T>::to_f(x[target]) : 0.f;
+  VocabStats st = vocab_thread_stats<T, THREADS, 4, ENTROPY, false>(x, r, part, scale);
+  uint32_t mine = 0;
+  if constexpr (TOP) mine = vocab_mine<T, THREADS>(x, r, part, st);
+  vocab_reduce<THREADS, ENTROPY>(st, scale, scratch, parts);
+  if (lead) {
+    if (a.Logp) a.Logp[row] = has ? vocab_logp(xt, st, a.temperature) : 0.f;
+    if (a.Entropy) a.Entropy[row] = vocab_entropy(st);
+    if (a.Mx) { a.Mx[row] = st.m; a.L[row] = st.s; }
+  }
+  if constexpr (TOP) {
+    __shared__ TopScratch<THREADS> top;
+    const int n = vocab_top<T, THREADS>(x, r, part, a.top, mine, top);
+    vocab_ranked<THREADS>(top, n, a.top, parts, [&](int rank, uint64_t key) {
+      a.TopLogp[row * a.top + rank] = vocab_logp(vocab_unkey((uint32_t)(key >> 32)), st, a.temperature);
+      a.TopIndex[row * a.top + rank] = vocab_key_index(key);
+    });
+  }
+  cluster_done(parts);
+}
+
+// Value and gradient.  GROUPS > 0: the part waits in shared memory for the second look; 0: it is read again, out of L2 as far as it is
+// still there.
+template <typename T, int THREADS, int U, int GROUPS, bool ENTROPY>
+__global__ void __launch_bounds__(THREADS, THREADS == 128 ? 8 : THREADS == 256 ? 5 : GROUPS ? 2 : 3)
+logprob_fwd_bwd_kernel(const LogprobArgs a, int parts) {
+  extern __shared__ uint4 kept[];
   __shared__ float scratch[100];
   const size_t row = blockIdx.x / parts;
   const T* x = (const T*)a.X + row * a.ldx;
@@ -66,29 +110,18 @@ __global__ void __launch_bounds__(THREADS, logprob_ctas(THREADS, ENTROPY, TOP, G
   const float scale = kVocabLog2e / a.temperature;
   const int target = a.targets ? a.targets[row] : -1;
   const bool has = target >= 0 && target < a.M;
-  const float xt = has ? Elem<T>::to_f(x[target]) : 0.f;
-  VocabStats st = vocab_thread_stats<T, THREADS, 4, ENTROPY, GRAD>(x, r, part, scale);
-  uint32_t mine = 0;
-  if constexpr (TOP) mine = vocab_mine<T, THREADS>(x, r, part, st);
+  const float xt = has ? Elem<T>::to_f(x[target]) : 0.f, g = has ? a.dLogp[row] : 0.f, h = ENTROPY && a.dEntropy ? a.dEntropy[row] : 0.f;
+  VocabStats st;
+  if constexpr (GROUPS > 0) st = vocab_resident_stats<T, THREADS, U, GROUPS, ENTROPY>(kept, x, r, part, scale);
+  else st = vocab_thread_stats<T, THREADS, U, ENTROPY, true>(x, r, part, scale);
   vocab_reduce<THREADS, ENTROPY>(st, scale, scratch, parts);
-  const float logL = st.s == 0.f ? 0.f : logf(st.s), H = st.s == 0.f ? 0.f : logL - kVocabLn2 * st.a / st.s;
-  const float mo = st.m == -INFINITY ? 0.f : st.m;
+  float H = 0.f;
+  if constexpr (ENTROPY) H = vocab_entropy(st);
   if (threadIdx.x == 0 && part.part == 0) {
-    if (a.Logp) a.Logp[row] = has ? (xt - mo) / a.temperature - logL : 0.f;
+    if (a.Logp) a.Logp[row] = has ? vocab_logp(xt, st, a.temperature) : 0.f;
     if (a.Entropy) a.Entropy[row] = H;
-    if (a.Mx) { a.Mx[row] = st.m; a.L[row] = st.s; }
   }
-  if constexpr (TOP) {
-    __shared__ TopScratch<THREADS> top;
-    const int n = vocab_top<T, THREADS>(x, r, part, a.top, mine, top);
-    vocab_ranked<THREADS>(top, n, a.top, parts, [&](int rank, uint64_t key) {
-      a.TopLogp[row * a.top + rank] = (vocab_unkey((uint32_t)(key >> 32)) - mo) / a.temperature - logL;
-      a.TopIndex[row * a.top + rank] = vocab_key_index(key);
-    });
-  }
-  if constexpr (GRAD)
-    logprob_part_grad<T, THREADS, ENTROPY>(a, row, x, r, part, has ? target : -1, xt, st.m, st.s, has ? a.dLogp[row] : 0.f,
-                                           ENTROPY && a.dEntropy ? a.dEntropy[row] : 0.f, H);
+  logprob_part_grad<T, THREADS, U, ENTROPY>(a, row, x, GROUPS > 0 ? kept : nullptr, r, part, has ? target : -1, xt, st.m, st.s, g, h, H);
   cluster_done(parts);
 }
 
@@ -102,24 +135,29 @@ __global__ void __launch_bounds__(THREADS, 6) logprob_bwd_kernel(const LogprobAr
   const bool has = target >= 0 && target < a.M;
   const float xt = has ? Elem<T>::to_f(x[target]) : 0.f;
   // (in place: the thread that uses xt is the one that writes its packet, later)
-  logprob_part_grad<T, THREADS, ENTROPY>(a, row, x, r, part, has ? target : -1, xt, a.inMx[row], a.inL[row], has ? a.dLogp[row] : 0.f,
+  logprob_part_grad<T, THREADS, 4, ENTROPY>(a, row, x, nullptr, r, part, has ? target : -1, xt, a.inMx[row], a.inL[row], has ? a.dLogp[row] : 0.f,
                                          ENTROPY ? a.dEntropy[row] : 0.f, ENTROPY ? a.inEntropy[row] : 0.f);
 }
 
-template <typename T, int THREADS, bool ENTROPY, bool GRAD>
-static int32_t logprob_launch(const char* who, const LogprobArgs& a, int64_t N, cudaStream_t stream) {
-  const int parts = vocab_parts(N, a.M / Elem<T>::kVec, THREADS);
-  if constexpr (!GRAD)
-    if (a.top) return launch_vocab(who, logprob_row_kernel<T, THREADS, ENTROPY, true, false>, a, N, parts, THREADS, stream);
-  return launch_vocab(who, logprob_row_kernel<T, THREADS, ENTROPY, false, GRAD>, a, N, parts, THREADS, stream);
+template <typename T, bool ENTROPY>
+static int32_t logprob_fwd_dispatch(const char* who, const LogprobArgs& a, int64_t N, cudaStream_t stream) {
+  const int64_t packets = a.M / Elem<T>::kVec;
+  const int parts = vocab_parts(N, packets);
+#define TYLO_FWD(THREADS, TOP) launch_vocab(who, logprob_fwd_kernel<T, THREADS, ENTROPY, TOP>, a, N, parts, THREADS, stream)
+  if (packets <= 1024) return a.top ? TYLO_FWD(128, true) : TYLO_FWD(128, false);
+  return a.top ? TYLO_FWD(512, true) : TYLO_FWD(512, false);
+#undef TYLO_FWD
 }
 
-template <typename T, bool GRAD>
-static int32_t logprob_dispatch(const char* who, const LogprobArgs& a, int64_t N, cudaStream_t stream) {
-  const bool entropy = a.Entropy || a.dEntropy;
-  if (a.M / Elem<T>::kVec <= 1024)
-    return entropy ? logprob_launch<T, 128, true, GRAD>(who, a, N, stream) : logprob_launch<T, 128, false, GRAD>(who, a, N, stream);
-  return entropy ? logprob_launch<T, 512, true, GRAD>(who, a, N, stream) : logprob_launch<T, 512, false, GRAD>(who, a, N, stream);
+template <typename T, bool ENTROPY>
+static int32_t logprob_fwd_bwd_dispatch(const char* who, const LogprobArgs& a, int64_t N, cudaStream_t stream) {
+  const int64_t packets = a.M / Elem<T>::kVec;
+  const int parts = vocab_parts(N, packets);
+  const int64_t per = (packets + parts - 1) / parts;
+#define TYLO_BOTH(THREADS, U, GROUPS) \
+  launch_vocab(who, logprob_fwd_bwd_kernel<T, THREADS, U, GROUPS, ENTROPY>, a, N, parts, THREADS, stream, GROUPS ? (int)per * 16 : 0)
+  TYLO_VOCAB_RESIDENT(TYLO_BOTH);
+#undef TYLO_BOTH
 }
 
 template <typename T>
@@ -151,7 +189,8 @@ extern "C" int32_t tylo_b200_token_logprobs_fwd(float* Logp, float* Entropy, flo
   LogprobArgs a = {};
   a.X = X; a.targets = targets; a.Logp = Logp; a.Entropy = Entropy; a.TopLogp = TopLogp; a.TopIndex = TopIndex; a.Mx = Mx; a.L = L;
   a.ldx = ldx; a.M = (int)M; a.top = top; a.temperature = temperature;
-  TYLO_DISPATCH_DTYPE(dtype, T, return (logprob_dispatch<T, false>(who, a, N, (cudaStream_t)stream)));
+  TYLO_DISPATCH_DTYPE(dtype, T, return (Entropy ? logprob_fwd_dispatch<T, true>(who, a, N, (cudaStream_t)stream)
+                                                : logprob_fwd_dispatch<T, false>(who, a, N, (cudaStream_t)stream)));
   return TYLO_OK;
 }
 
@@ -189,6 +228,7 @@ extern "C" int32_t tylo_b200_token_logprobs_fwd_bwd(float* Logp, float* Entropy,
   LogprobArgs a = {};
   a.X = X; a.targets = targets; a.Logp = Logp; a.Entropy = Entropy; a.dX = dX; a.dLogp = dLogp; a.dEntropy = dEntropy;
   a.ldx = ldx; a.M = (int)M; a.temperature = temperature;
-  TYLO_DISPATCH_DTYPE(dtype, T, return (logprob_dispatch<T, true>(who, a, N, (cudaStream_t)stream)));
+  TYLO_DISPATCH_DTYPE(dtype, T, return (Entropy || dEntropy ? logprob_fwd_bwd_dispatch<T, true>(who, a, N, (cudaStream_t)stream)
+                                                            : logprob_fwd_bwd_dispatch<T, false>(who, a, N, (cudaStream_t)stream)));
   return TYLO_OK;
 }

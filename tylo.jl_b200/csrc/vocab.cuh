@@ -169,21 +169,17 @@ template <typename T> __device__ __forceinline__ uint4 no_logits() {
   return make_uint4(w, w, w, w);
 }
 
-// One thread's share of a part: every THREADS-th packet, U at a time, and a single element.  Sums are kept in two chains (packed fp32
-// pairs).  KEEP: the part will be read again.
-template <typename T, int THREADS, int U, bool ENTROPY, bool KEEP>
-__device__ __forceinline__ VocabStats vocab_thread_stats(const T* x, const VocabRow<T>& r, const VocabPart& part, float scale) {
-  constexpr int VEC = Elem<T>::kVec;
+// One thread's running sums, in two chains (packed fp32 pairs).
+template <typename T, bool ENTROPY> struct VocabSum {
+  static constexpr int kVec = Elem<T>::kVec;
   float m = -INFINITY, ref = -INFINITY;
-  float2 s = make_float2(0.f, 0.f), a = s;
-  const int one = part.part == 0 ? r.single(threadIdx.x) : -1;
-  if (one >= 0) {                                   // (a NaN or +Inf gives a NaN sum here as below)
-    const float f = Elem<T>::to_f(x[one]);
+  float2 s = {0.f, 0.f}, a = {0.f, 0.f};
+
+  __device__ __forceinline__ void first(float f, float scale) {       // a single element (a NaN or +Inf gives a NaN sum here as below)
     m = ref = fmaxf(m, f);
     s.x = vocab_ex2((f - (ref == -INFINITY ? 0.f : ref)) * scale);
   }
-  const float2 sc = make_float2(scale, scale);
-  auto take = [&](const Pack<T> (&p)[U]) {
+  template <int U> __device__ __forceinline__ void take(const Pack<T> (&p)[U], float scale) {
     m = fmaxf(m, packets_max<T, U>(p));
     if ((m - ref) * scale > kRefSlack) {              // (both -Inf: a NaN, no)
       const float d = fmaxf((ref - m) * scale, kExpFloor), e = vocab_ex2(d);
@@ -192,20 +188,30 @@ __device__ __forceinline__ VocabStats vocab_thread_stats(const T* x, const Vocab
       ref = m;
     }
     const float mo = ref == -INFINITY ? 0.f : -ref;
-    const float2 nm = make_float2(mo, mo);
+    const float2 nm = make_float2(mo, mo), sc = make_float2(scale, scale);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      float f[VEC];
+      float f[kVec];
       p[u].unpack(f);
 #pragma unroll
-      for (int j = 0; j < VEC; j += 2) {
+      for (int j = 0; j < kVec; j += 2) {
         const float2 y = __fmul2_rn(__fadd2_rn(make_float2(f[j], f[j + 1]), nm), sc);
         const float2 e = make_float2(vocab_ex2(y.x), vocab_ex2(y.y));
         s = __fadd2_rn(s, e);
         if constexpr (ENTROPY) a = __ffma2_rn(e, make_float2(fmaxf(y.x, kExpFloor), fmaxf(y.y, kExpFloor)), a);
       }
     }
-  };
+  }
+  __device__ __forceinline__ VocabStats stats() const { return {m, ref, s.x + s.y, a.x + a.y}; }
+};
+
+// One thread's share of a part: every THREADS-th packet, U at a time, and a single element.  KEEP: the part will be read again.
+template <typename T, int THREADS, int U, bool ENTROPY, bool KEEP>
+__device__ __forceinline__ VocabStats vocab_thread_stats(const T* x, const VocabRow<T>& r, const VocabPart& part, float scale) {
+  constexpr int VEC = Elem<T>::kVec;
+  VocabSum<T, ENTROPY> sum;
+  const int one = part.part == 0 ? r.single(threadIdx.x) : -1;
+  if (one >= 0) sum.first(Elem<T>::to_f(x[one]), scale);
   const uint64_t keep = KEEP ? keep_policy() : 0;
   const T* q = x + r.index(part.lo + threadIdx.x);
   auto load = [&](Pack<T>& p, int u) {
@@ -217,7 +223,7 @@ __device__ __forceinline__ VocabStats vocab_thread_stats(const T* x, const Vocab
   for (; left > (U - 1) * THREADS; left -= U * THREADS, q += U * THREADS * VEC) {
 #pragma unroll
     for (int u = 0; u < U; ++u) load(p[u], u);
-    take(p);
+    sum.take(p, scale);
   }
   if (left > 0) {
 #pragma unroll
@@ -225,13 +231,84 @@ __device__ __forceinline__ VocabStats vocab_thread_stats(const T* x, const Vocab
       if (left > u * THREADS) load(p[u], u);
       else p[u].raw = no_logits<T>();
     }
-    take(p);
+    sum.take(p, scale);
   }
-  return {m, ref, s.x + s.y, a.x + a.y};
+  return sum.stats();
 }
 
-// Gradient of a part: f(pair of logits) -> pair of gradients for every element, rounded once, on the way out.  As the second look at a
-// part it goes backwards: what was read last is the likeliest to be in L2.
+// The same for a part of at most THREADS * U * GROUPS packets that waits in shared memory for its second look.  Every thread asks for
+// all of its packets at once, by asynchronous copies in GROUPS groups, and reads back nothing but its own: no barrier, no registers
+// held by what is on its way.
+__device__ __forceinline__ void wait_copies(int later) {       // until at most `later` groups of this thread's copies are on their way
+  switch (later) {
+#define TYLO_WAIT_COPIES(N) case N: asm volatile("cp.async.wait_group " #N ";" ::: "memory"); break;
+    TYLO_WAIT_COPIES(0) TYLO_WAIT_COPIES(1) TYLO_WAIT_COPIES(2) TYLO_WAIT_COPIES(3)
+    TYLO_WAIT_COPIES(4) TYLO_WAIT_COPIES(5) TYLO_WAIT_COPIES(6) TYLO_WAIT_COPIES(7)
+#undef TYLO_WAIT_COPIES
+  }
+}
+template <typename T, int THREADS, int U, int GROUPS, bool ENTROPY>
+__device__ __forceinline__ VocabStats vocab_resident_stats(uint4* row, const T* x, const VocabRow<T>& r, const VocabPart& part, float scale) {
+  static_assert(GROUPS <= 8, "wait_copies");
+  constexpr int VEC = Elem<T>::kVec;
+  const int n = part.hi - part.lo - (int)threadIdx.x;          // this thread's packet k * THREADS is there if n > k * THREADS
+  const T* q = x + r.index(part.lo + threadIdx.x);
+  uint4* own = row + threadIdx.x;
+  const uint32_t to = (uint32_t)__cvta_generic_to_shared(own);
+#pragma unroll
+  for (int g = 0; g < GROUPS; ++g) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = (g * U + u) * THREADS;
+      if (n > k) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + k * 16), "l"(q + k * VEC) : "memory");
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  VocabSum<T, ENTROPY> sum;
+  const int one = part.part == 0 ? r.single(threadIdx.x) : -1;
+  if (one >= 0) sum.first(Elem<T>::to_f(x[one]), scale);
+#pragma unroll
+  for (int g = 0; g < GROUPS; ++g) {
+    wait_copies(GROUPS - 1 - g);
+    if (n > g * U * THREADS) {
+      Pack<T> p[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int k = (g * U + u) * THREADS;
+        p[u].raw = n > k ? own[k] : no_logits<T>();
+      }
+      sum.take(p, scale);
+    }
+  }
+  return sum.stats();
+}
+
+// Gradient of a part that waits in shared memory (vocab_resident_stats): f(pair of logits) -> pair of gradients for every element,
+// rounded once, on the way out.
+template <typename T, int THREADS, int U, typename F>
+__device__ __forceinline__ void vocab_resident_rewrite(T* dx, const uint4* kept, const T* x, const VocabRow<T>& r, const VocabPart& part, F f) {
+  constexpr int VEC = Elem<T>::kVec;
+  const int one = part.part == 0 ? r.single(threadIdx.x) : -1;
+  if (one >= 0) dx[one] = Elem<T>::from_f(f(make_float2(Elem<T>::to_f(x[one]), 0.f)).x);
+  const int n = part.hi - part.lo;
+  T* to = dx + r.index(part.lo);
+#pragma unroll U
+  for (int v = threadIdx.x; v < n; v += THREADS) {
+    Pack<T> p;
+    p.raw = kept[v];
+    float e[VEC];
+    p.unpack(e);
+#pragma unroll
+    for (int j = 0; j < VEC; j += 2) {
+      const float2 d = f(make_float2(e[j], e[j + 1]));
+      e[j] = d.x; e[j + 1] = d.y;
+    }
+    p.pack(e);
+    st_stream(to + (size_t)v * VEC, p.raw);
+  }
+}
+
+// The same from global memory.  As the second look at a part it goes backwards: what was read last is the likeliest to be in L2.
 template <typename T, int THREADS, int U, typename F>
 __device__ __forceinline__ void vocab_rewrite(T* dx, const T* x, const VocabRow<T>& r, const VocabPart& part, F f) {
   constexpr int VEC = Elem<T>::kVec;
@@ -584,10 +661,13 @@ __device__ __forceinline__ uint32_t vocab_mine(const T* x, const VocabRow<T>& r,
 
 // Launches `parts` CTAs per row, as a cluster where they have something to tell one another.
 template <typename A>
-int32_t launch_vocab(const char* who, void (*kernel)(A, int), const A& args, int64_t N, int parts, int threads, cudaStream_t stream) {
+int32_t launch_vocab(const char* who, void (*kernel)(A, int), const A& args, int64_t N, int parts, int threads, cudaStream_t stream, int smem = 0) {
+  if (smem > 40 * 1024)       // (with the kernels' own arrays; the default limit is 48 KB)
+    TYLO_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(N * parts));
   cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -600,11 +680,20 @@ int32_t launch_vocab(const char* who, void (*kernel)(A, int), const A& args, int
 }
 
 // CTAs per row: a row is dealt over a cluster while rows alone leave SMs without a CTA.
-inline int vocab_parts(int64_t N, int64_t packets, int threads) {
+inline int vocab_parts(int64_t N, int64_t packets, int64_t least = 1024) {
   int parts = 1;
-  while (parts < 8 && N * parts * 2 <= 2 * sm_count() && packets >= 2LL * parts * threads) parts *= 2;
+  while (parts < 8 && N * parts * 2 <= 2 * sm_count() && packets >= parts * least) parts *= 2;
   return parts;
 }
+
+// Shape of a kernel that looks at its row twice: rows of up to kResident packets per CTA wait in shared memory.
+constexpr int kResident = 6784;           // 106 KB: two CTAs per SM
+#define TYLO_VOCAB_RESIDENT(LAUNCH)                                      \
+  if (per <= 1024) return LAUNCH(128, 4, 2);                             \
+  if (per <= 2048) return LAUNCH(128, 4, 4);                             \
+  if (per <= 4096) return LAUNCH(256, 4, 4);                             \
+  if (per <= kResident) return LAUNCH(512, 2, 7);                        \
+  return LAUNCH(512, 4, 0)
 
 inline int32_t check_vocab(const char* who, const void* X, int64_t M, int64_t N, int64_t ldx, float temperature) {
   TYLO_REQUIRE(X, TYLO_ERR_INVALID_ARGUMENT, "%s: X must be non-null", who);
