@@ -73,10 +73,10 @@ __global__ void __launch_bounds__(THREADS, logprob_ctas(THREADS, ENTROPY, TOP)) 
   const VocabPart part(blockIdx.x % parts, parts, r.whole);
   const float scale = kVocabLog2e / a.temperature;
   const bool lead = threadIdx.x == 0 && part.part == 0;
-  const int target = lead && a.Logp ? a.targets[row] : -1;
+  const int target = lead && a.Logp ? a.targets[row] : -1;       // (first used behind the sums: nothing waits for it here)
+  VocabStats st = vocab_thread_stats<T, THREADS, 4, ENTROPY, false>(x, r, part, scale);
   const bool has = target >= 0 && target < a.M;
   const float xt = has ? Elem<T>::to_f(x[target]) : 0.f;
-  VocabStats st = vocab_thread_stats<T, THREADS, 4, ENTROPY, false>(x, r, part, scale);
   uint32_t mine = 0;
   if constexpr (TOP) mine = vocab_mine<T, THREADS>(x, r, part, st);
   vocab_reduce<THREADS, ENTROPY>(st, scale, scratch, parts);
@@ -108,12 +108,15 @@ logprob_fwd_bwd_kernel(const LogprobArgs a, int parts) {
   const VocabRow<T> r(x, a.M);
   const VocabPart part(blockIdx.x % parts, parts, r.whole);
   const float scale = kVocabLog2e / a.temperature;
-  const int target = a.targets ? a.targets[row] : -1;
-  const bool has = target >= 0 && target < a.M;
-  const float xt = has ? Elem<T>::to_f(x[target]) : 0.f, g = has ? a.dLogp[row] : 0.f, h = ENTROPY && a.dEntropy ? a.dEntropy[row] : 0.f;
+  const int target = a.targets ? a.targets[row] : -1;            // (first used behind the sums: nothing waits for these here)
+  float g = a.targets ? a.dLogp[row] : 0.f;
+  const float h = ENTROPY && a.dEntropy ? a.dEntropy[row] : 0.f;
   VocabStats st;
   if constexpr (GROUPS > 0) st = vocab_resident_stats<T, THREADS, U, GROUPS, ENTROPY>(kept, x, r, part, scale);
   else st = vocab_thread_stats<T, THREADS, U, ENTROPY, true>(x, r, part, scale);
+  const bool has = target >= 0 && target < a.M;
+  const float xt = has ? Elem<T>::to_f(x[target]) : 0.f;
+  g = has ? g : 0.f;
   vocab_reduce<THREADS, ENTROPY>(st, scale, scratch, parts);
   float H = 0.f;
   if constexpr (ENTROPY) H = vocab_entropy(st);
