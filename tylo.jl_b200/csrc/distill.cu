@@ -76,7 +76,7 @@ distill_row_kernel(const DistillArgs a, int parts) {
   const float it = 1.f / a.temperature, scale = kVocabLog2e / a.temperature;
   VocabStats st;
   if constexpr (GROUPS > 0) st = vocab_resident_stats<T, THREADS, U, GROUPS, false>(kept, x, r, part, scale);
-  else if constexpr (LOSS) st = vocab_thread_stats<T, THREADS, U, false, GRAD>(x, r, part, scale);
+  else if constexpr (LOSS) st = vocab_thread_stats<T, THREADS, U, false, GRAD, false>(x, r, part, scale, nullptr);
   float mass;
   const float log_norm = teacher_row<THREADS>(a, row, p, index, scratch, mass);
   for (int k = threadIdx.x; k < a.K; k += THREADS) xk[k] = index[k] >= 0 ? Elem<T>::to_f(x[index[k]]) : 0.f;

@@ -62,7 +62,7 @@ __device__ __forceinline__ void logprob_part_grad(const LogprobArgs& a, size_t r
 }
 
 // CTAs per SM: registers for as many as the loads need to be hidden behind one another, or as shared memory holds
-constexpr int logprob_ctas(int threads, bool entropy, bool top) { return (threads == 128 ? 4 : 1) * (top ? 2 : entropy ? 3 : 4); }
+constexpr int logprob_ctas(int threads, bool entropy, bool top) { return 512 / threads * (top ? 2 : entropy ? 3 : 4); }
 
 template <typename T, int THREADS, bool ENTROPY, bool TOP>
 __global__ void __launch_bounds__(THREADS, logprob_ctas(THREADS, ENTROPY, TOP)) logprob_fwd_kernel(const LogprobArgs a, int parts) {
@@ -74,11 +74,14 @@ __global__ void __launch_bounds__(THREADS, logprob_ctas(THREADS, ENTROPY, TOP)) 
   const float scale = kVocabLog2e / a.temperature;
   const bool lead = threadIdx.x == 0 && part.part == 0;
   const int target = lead && a.Logp ? a.targets[row] : -1;       // (first used behind the sums: nothing waits for it here)
-  VocabStats st = vocab_thread_stats<T, THREADS, 4, ENTROPY, false>(x, r, part, scale);
+  extern __shared__ ulonglong2 top_space[];
+  TopScratch<THREADS>& top = *reinterpret_cast<TopScratch<THREADS>*>(top_space);
+  const VocabCells<THREADS> cells(TOP ? top.cells : nullptr, part.hi - part.lo, 4 * THREADS);
+  VocabStats st = vocab_thread_stats<T, THREADS, 4, ENTROPY, false, TOP>(x, r, part, scale, &cells);
   const bool has = target >= 0 && target < a.M;
   const float xt = has ? Elem<T>::to_f(x[target]) : 0.f;
-  uint32_t mine = 0;
-  if constexpr (TOP) mine = vocab_mine<T, THREADS>(x, r, part, st);
+  const bool odd = st.s != st.s;
+  if constexpr (TOP) top.mine[threadIdx.x] = vocab_mine<T, THREADS>(x, r, part, st);
   vocab_reduce<THREADS, ENTROPY>(st, scale, scratch, parts);
   if (lead) {
     if (a.Logp) a.Logp[row] = has ? vocab_logp(xt, st, a.temperature) : 0.f;
@@ -86,8 +89,7 @@ __global__ void __launch_bounds__(THREADS, logprob_ctas(THREADS, ENTROPY, TOP)) 
     if (a.Mx) { a.Mx[row] = st.m; a.L[row] = st.s; }
   }
   if constexpr (TOP) {
-    __shared__ TopScratch<THREADS> top;
-    const int n = vocab_top<T, THREADS>(x, r, part, a.top, mine, top);
+    const int n = vocab_top<T, THREADS, 4>(x, r, part, a.top, cells, odd, top);
     vocab_ranked<THREADS>(top, n, a.top, parts, [&](int rank, uint64_t key) {
       a.TopLogp[row * a.top + rank] = vocab_logp(vocab_unkey((uint32_t)(key >> 32)), st, a.temperature);
       a.TopIndex[row * a.top + rank] = vocab_key_index(key);
@@ -113,7 +115,7 @@ logprob_fwd_bwd_kernel(const LogprobArgs a, int parts) {
   const float h = ENTROPY && a.dEntropy ? a.dEntropy[row] : 0.f;
   VocabStats st;
   if constexpr (GROUPS > 0) st = vocab_resident_stats<T, THREADS, U, GROUPS, ENTROPY>(kept, x, r, part, scale);
-  else st = vocab_thread_stats<T, THREADS, U, ENTROPY, true>(x, r, part, scale);
+  else st = vocab_thread_stats<T, THREADS, U, ENTROPY, true, false>(x, r, part, scale, nullptr);
   const bool has = target >= 0 && target < a.M;
   const float xt = has ? Elem<T>::to_f(x[target]) : 0.f;
   g = has ? g : 0.f;
@@ -146,9 +148,13 @@ template <typename T, bool ENTROPY>
 static int32_t logprob_fwd_dispatch(const char* who, const LogprobArgs& a, int64_t N, cudaStream_t stream) {
   const int64_t packets = a.M / Elem<T>::kVec;
   const int parts = vocab_parts(N, packets);
-#define TYLO_FWD(THREADS, TOP) launch_vocab(who, logprob_fwd_kernel<T, THREADS, ENTROPY, TOP>, a, N, parts, THREADS, stream)
-  if (packets <= 1024) return a.top ? TYLO_FWD(128, true) : TYLO_FWD(128, false);
-  return a.top ? TYLO_FWD(512, true) : TYLO_FWD(512, false);
+#define TYLO_FWD(THREADS, TOP) \
+  launch_vocab(who, logprob_fwd_kernel<T, THREADS, ENTROPY, TOP>, a, N, parts, THREADS, stream, TOP ? (int)sizeof(TopScratch<THREADS>) : 0)
+  const int64_t per = (packets + parts - 1) / parts;
+  if (a.top) return a.top <= 64 ? TYLO_FWD(256, true) : TYLO_FWD(512, true);
+  if (per <= 2048) return TYLO_FWD(128, false);
+  if (per <= 8192) return TYLO_FWD(256, false);
+  return TYLO_FWD(512, false);
 #undef TYLO_FWD
 }
 

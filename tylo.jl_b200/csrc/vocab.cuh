@@ -179,8 +179,9 @@ template <typename T, bool ENTROPY> struct VocabSum {
     m = ref = fmaxf(m, f);
     s.x = vocab_ex2((f - (ref == -INFINITY ? 0.f : ref)) * scale);
   }
-  template <int U> __device__ __forceinline__ void take(const Pack<T> (&p)[U], float scale) {
-    m = fmaxf(m, packets_max<T, U>(p));
+  template <int U> __device__ __forceinline__ float take(const Pack<T> (&p)[U], float scale) {       // returns the largest of the step
+    const float most = packets_max<T, U>(p);
+    m = fmaxf(m, most);
     if ((m - ref) * scale > kRefSlack) {              // (both -Inf: a NaN, no)
       const float d = fmaxf((ref - m) * scale, kExpFloor), e = vocab_ex2(d);
       if constexpr (ENTROPY) a = __fmul2_rn(make_float2(e, e), __ffma2_rn(make_float2(d, d), s, a));
@@ -201,13 +202,28 @@ template <typename T, bool ENTROPY> struct VocabSum {
         if constexpr (ENTROPY) a = __ffma2_rn(e, make_float2(fmaxf(y.x, kExpFloor), fmaxf(y.y, kExpFloor)), a);
       }
     }
+    return most;
   }
   __device__ __forceinline__ VocabStats stats() const { return {m, ref, s.x + s.y, a.x + a.y}; }
 };
 
+// The largest logit of every cell of a thread's share: a cell is 2^shift consecutive steps, so that no share has more than kCells.
+constexpr int kCells = 16;
+template <int THREADS> struct VocabCells {
+  float (*max)[THREADS];       // shared memory: kCells rows
+  int shift, cells;
+  __device__ __forceinline__ VocabCells(float (*max_)[THREADS], int packets, int per_step) : max(max_), shift(0) {
+    const int steps = (packets + per_step - 1) / per_step;
+    while ((steps - 1) >> shift >= kCells) ++shift;
+    cells = steps > 0 ? ((steps - 1) >> shift) + 1 : 0;
+  }
+};
+
 // One thread's share of a part: every THREADS-th packet, U at a time, and a single element.  KEEP: the part will be read again.
-template <typename T, int THREADS, int U, bool ENTROPY, bool KEEP>
-__device__ __forceinline__ VocabStats vocab_thread_stats(const T* x, const VocabRow<T>& r, const VocabPart& part, float scale) {
+// CELLS: the largest logits of the cells are left in `cells` (the single element belongs to none).
+template <typename T, int THREADS, int U, bool ENTROPY, bool KEEP, bool CELLS>
+__device__ __forceinline__ VocabStats vocab_thread_stats(const T* x, const VocabRow<T>& r, const VocabPart& part, float scale,
+                                                         const VocabCells<THREADS>* cells) {
   constexpr int VEC = Elem<T>::kVec;
   VocabSum<T, ENTROPY> sum;
   const int one = part.part == 0 ? r.single(threadIdx.x) : -1;
@@ -220,6 +236,24 @@ __device__ __forceinline__ VocabStats vocab_thread_stats(const T* x, const Vocab
   };
   int left = part.hi - part.lo - (int)threadIdx.x;    // packets from this thread's next one to the part's end
   Pack<T> p[U];
+  if constexpr (CELLS) {
+    float most = -INFINITY;
+    for (int c = 0, i = 0; c < cells->cells; ++i, left -= U * THREADS, q += U * THREADS * VEC) {
+      if (left > 0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (left > u * THREADS) load(p[u], u);
+          else p[u].raw = no_logits<T>();
+        }
+        most = fmaxf(most, sum.take(p, scale));
+      }
+      if (((i + 1) & ((1 << cells->shift) - 1)) == 0 || (int)(left + threadIdx.x) <= U * THREADS) {     // the cell's, or the part's, last step
+        cells->max[c++][threadIdx.x] = most;
+        most = -INFINITY;
+      }
+    }
+    return sum.stats();
+  }
   for (; left > (U - 1) * THREADS; left -= U * THREADS, q += U * THREADS * VEC) {
 #pragma unroll
     for (int u = 0; u < U; ++u) load(p[u], u);
@@ -373,20 +407,21 @@ __device__ __forceinline__ int vocab_key_index(uint64_t k) { return 0x7fffffff -
 
 // ---- the largest elements of a part ------------------------------------------------------------------------------------------
 // A bound first: the K-th largest of the threads' own maxima, which the statistics leave behind, is no larger than the K-th largest
-// element, and no more than K threads (and ties) have anything to show above it.  Only those read their elements again, out of L2,
-// and put what reaches the bound into shared memory: little more than K elements unless they sit together in few threads' shares or
-// are equal.  Where they do not fit, the bound is raised by counting, and equal elements at the bound are taken in the order of
-// their index.  What is left is thinned by bisection to K and a few, whose rank is counted.
+// element, and little more than K cells of all threads reach it.  Only those are read again, out of L2, and what reaches the bound goes
+// to shared memory: little more than K elements unless many sit together in few shares or are equal.  Where they do not fit, the bound
+// is raised by counting, and equal elements at the bound are taken in the order of their index.  What is left is thinned by bisection
+// to K and a few, whose rank is counted.
 constexpr int kTopSlack = 32;
 
 template <int THREADS> struct TopScratch {
-  static constexpr int kSlots = 8 * THREADS;
-  uint64_t keys[kSlots];
-  uint64_t few[TYLO_TOP_MAX + kTopSlack];
+  static constexpr int kSlots = 4 * THREADS;
+  ulonglong2 keys2[kSlots / 2], few2[(TYLO_TOP_MAX + kTopSlack) / 2];
   uint64_t sorted[TYLO_TOP_MAX];
-  uint32_t warp[64];
-  uint16_t who[THREADS];
-  int n, m, w;
+  float cells[kCells][THREADS];
+  uint32_t mine[THREADS];                 // the threads' largest elements as keys
+  uint32_t warp[64], bound, most;
+  uint16_t hits[THREADS / 32][64];
+  int n, m;
 };
 
 template <int THREADS> struct BlockCount {
@@ -405,70 +440,97 @@ template <int THREADS> struct BlockCount {
 };
 
 // Puts the min(K, elements of the part) largest elements of the part into sc.sorted, in falling order, and returns how many.
-// `mine`: this thread's largest element as a key, 0 without elements.
-template <typename T, int THREADS>
-__device__ __noinline__ int vocab_top(const T* x, const VocabRow<T> r, const VocabPart part, int K, uint32_t mine, TopScratch<THREADS>& sc) {
+// sc.mine[thread]: the thread's largest element as a key, 0 without elements, written before a barrier of the CTA; `cells`: see
+// vocab_thread_stats<U>; `all`: this thread's cells cannot be relied on (a NaN, which their maxima pass over).
+template <typename T, int THREADS, int U>
+__device__ __noinline__ int vocab_top(const T* x, const VocabRow<T> r, const VocabPart part, int K, VocabCells<THREADS> cells, bool all,
+                                      TopScratch<THREADS>& sc) {
   constexpr int VEC = Elem<T>::kVec, kTopSlots = TopScratch<THREADS>::kSlots;
+  uint64_t *keys = reinterpret_cast<uint64_t*>(sc.keys2), *few = reinterpret_cast<uint64_t*>(sc.few2);
   const int elements = (part.hi - part.lo) * VEC + (part.part == 0 ? r.head + r.tail : 0);
   K = min(K, elements);
   BlockCount<THREADS> count{sc.warp, 0};
-  if (threadIdx.x == 0) { sc.n = 0; sc.m = 0; sc.w = 0; }
-  const int lane = threadIdx.x & 31;
-  // largest and smallest key among the threads that have one
-  uint32_t hi = __reduce_max_sync(0xffffffffu, mine), lo = __reduce_min_sync(0xffffffffu, mine ? mine : 0xffffffffu);
-  if (lane == 0) { sc.warp[threadIdx.x >> 5] = hi; sc.warp[32 + (threadIdx.x >> 5)] = lo; }
-  __syncthreads();
-  hi = __reduce_max_sync(0xffffffffu, lane < THREADS / 32 ? sc.warp[lane] : 0);
-  lo = __reduce_min_sync(0xffffffffu, lane < THREADS / 32 ? sc.warp[32 + lane] : 0xffffffffu);
-  const uint32_t top = hi;
-  uint32_t t = 1;                              // below every element
-  if (__syncthreads_count(mine != 0) >= K) {
-    while (lo < hi) {
-      const uint32_t mid = lo + (hi - lo) / 2 + 1;
-      const int c = __syncthreads_count(mine >= mid);
-      if (c >= K) {
-        lo = mid;
-        if (c <= K + K / 8) break;
-      } else {
-        hi = mid - 1;
-      }
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t mine = sc.mine[threadIdx.x];
+  if (warp == 0) {
+    // one warp looks for the bound, by bisection between the smallest and the largest maximum; an eighth more than K will do
+    uint32_t k[THREADS / 32], hi = 0, lo = 0xffffffffu;
+    int live = 0;
+#pragma unroll
+    for (int i = 0; i < THREADS / 32; ++i) {
+      k[i] = sc.mine[i * 32 + lane];
+      hi = max(hi, k[i]);
+      lo = min(lo, k[i] - 1);               // (0 becomes the largest)
+      live += k[i] != 0;
     }
-    t = lo;
+    hi = __reduce_max_sync(0xffffffffu, hi);
+    lo = __reduce_min_sync(0xffffffffu, lo) + 1;
+    const uint32_t most = hi;
+    if (__reduce_add_sync(0xffffffffu, live) >= K) {
+      while (lo < hi) {
+        const uint32_t mid = lo + (hi - lo) / 2 + 1;
+        int c = 0;
+#pragma unroll
+        for (int i = 0; i < THREADS / 32; ++i) c += k[i] >= mid;
+        c = __reduce_add_sync(0xffffffffu, c);
+        if (c >= K) {
+          lo = mid;
+          if (c <= K + K / 8) break;
+        } else {
+          hi = mid - 1;
+        }
+      }
+    } else {
+      lo = 1;                               // below every element
+    }
+    if (lane == 0) { sc.bound = lo; sc.most = most; sc.n = 0; sc.m = 0; }
   }
-  // Hands the elements of the threads whose maximum reaches `from` to f(values, number of values, first index) by the packet.  The
-  // packets of those threads are dealt over the whole CTA; f returns false when it has seen enough.
+  __syncthreads();
+  uint32_t t = sc.bound, lo, hi;
+  const uint32_t top = sc.most;
+  // Hands the elements of the cells whose maximum reaches `from` to f(values, number of values, first index) by the packet: a warp
+  // lists such cells of its threads and deals their packets over its lanes.  f returns false when it has seen enough.
   auto visit = [&](uint32_t from, auto f) {
-    if (mine >= from) sc.who[atomicAdd(&sc.w, 1)] = threadIdx.x;
-    __syncthreads();
-    const int w = sc.w, per = (part.hi - part.lo + THREADS - 1) / THREADS, all = w * per;
-    constexpr int U = 4;
     bool more = true;
-    const int one = part.part == 0 && mine >= from ? r.single(threadIdx.x) : -1;
+    const int one = part.part == 0 ? r.single(threadIdx.x) : -1;
     if (one >= 0) {
       float e[VEC];
       e[0] = Elem<T>::to_f(x[one]);
       more = f(e, 1, one);
     }
-    for (int i0 = threadIdx.x; i0 < all && more; i0 += U * THREADS) {
-      Pack<T> p[U];
-      int v[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int i = i0 + u * THREADS;
-        v[u] = i < all ? part.lo + sc.who[i % w] + i / w * THREADS : part.hi;
-        if (v[u] < part.hi) p[u].raw = ld_logits(x + r.index(v[u]));
+    if (__all_sync(0xffffffffu, mine < from)) return;
+    uint16_t* hits = sc.hits[warp];
+    static_assert(U == 4, "packets of a cell as a power of two");
+    const int lg = cells.shift + 2, per = 1 << lg;
+    for (int c = 0; c < cells.cells;) {
+      int n = 0;
+      for (; c < cells.cells && n <= 32; ++c) {
+        const bool hit = mine >= from && (all || vocab_key(cells.max[c][threadIdx.x]) >= from);
+        const uint32_t mask = __ballot_sync(0xffffffffu, hit);
+        if (hit) hits[n + __popc(mask & ((1u << lane) - 1))] = (uint16_t)(c * 32 + lane);
+        n += __popc(mask);
       }
+      __syncwarp();
+      for (int i0 = lane; i0 < n * per && more; i0 += 4 * 32) {
+        Pack<T> p[4];
+        int v[4];
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (v[u] < part.hi && more) {
-          float e[VEC];
-          p[u].unpack(e);
-          more = f(e, VEC, r.index(v[u]));
+        for (int u = 0; u < 4; ++u) {
+          const int i = i0 + u * 32, h = i < n * per ? hits[i >> lg] : 0;
+          v[u] = part.lo + ((h >> 5) * per + (i & (per - 1))) * THREADS + warp * 32 + (h & 31);
+          if (i >= n * per) v[u] = part.hi;
+          if (v[u] < part.hi) p[u].raw = ld_logits(x + r.index(v[u]));
         }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (v[u] < part.hi && more) {
+            float e[VEC];
+            p[u].unpack(e);
+            more = f(e, VEC, r.index(v[u]));
+          }
+      }
+      __syncwarp();
     }
-    __syncthreads();
-    if (threadIdx.x == 0) sc.w = 0;
-    __syncthreads();
   };
   // elements above or at a bound into sc.keys; more than kTopSlots: at least that many
   auto collect = [&](uint32_t from) {
@@ -486,11 +548,12 @@ __device__ __noinline__ int vocab_top(const T* x, const VocabRow<T> r, const Voc
 #pragma unroll
       for (int j = 0; j < VEC; ++j)
         if (hit >> j & 1) {
-          if (k < kTopSlots) sc.keys[k] = vocab_key(e[j], first + j);
+          if (k < kTopSlots) keys[k] = vocab_key(e[j], first + j);
           ++k;
         }
       return at < kTopSlots;
     });
+    __syncthreads();
     return sc.n;
   };
   auto at_least = [&](uint32_t from) {
@@ -552,7 +615,7 @@ __device__ __noinline__ int vocab_top(const T* x, const VocabRow<T> r, const Voc
         __syncthreads();
         int rank = taken + ahead + before - c;
         for (uint32_t b = ties; b && rank < need; b &= b - 1, ++rank)
-          sc.keys[n + rank] = ((uint64_t)t << 32) | (uint32_t)(0x7fffffff - (first + __ffs(b) - 1));
+          keys[n + rank] = ((uint64_t)t << 32) | (uint32_t)(0x7fffffff - (first + __ffs(b) - 1));
         taken += all;
       };
       if (part.part == 0 && r.head) block((int)threadIdx.x < r.head && vocab_key(Elem<T>::to_f(x[threadIdx.x])) == t, threadIdx.x);
@@ -576,15 +639,12 @@ __device__ __noinline__ int vocab_top(const T* x, const VocabRow<T> r, const Voc
     }
   }
   // n >= K different keys: thin them, then rank them
-  const uint64_t* list = sc.keys;
+  uint64_t* list = keys;
   if (n > K + kTopSlack) {
     constexpr int PER = kTopSlots / THREADS;
-    uint64_t mine64[PER], most = 0;
+    uint64_t mine64[PER];
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      mine64[i] = i * THREADS + threadIdx.x < n ? sc.keys[i * THREADS + threadIdx.x] : 0;
-      most = mine64[i] > most ? mine64[i] : most;
-    }
+    for (int i = 0; i < PER; ++i) mine64[i] = i * THREADS + threadIdx.x < n ? keys[i * THREADS + threadIdx.x] : 0;
     uint64_t lo64 = (uint64_t)t << 32, hi64 = ((uint64_t)top << 32) | 0xffffffffu;
     while (lo64 < hi64) {
       const uint64_t mid = lo64 + (hi64 - lo64) / 2 + 1;
@@ -601,16 +661,25 @@ __device__ __noinline__ int vocab_top(const T* x, const VocabRow<T> r, const Voc
     }
 #pragma unroll
     for (int i = 0; i < PER; ++i)
-      if (mine64[i] >= lo64) sc.few[atomicAdd(&sc.m, 1)] = mine64[i];
+      if (mine64[i] >= lo64) few[atomicAdd(&sc.m, 1)] = mine64[i];
     __syncthreads();
     n = sc.m;
-    list = sc.few;
+    list = few;
   }
-  for (int i = threadIdx.x; i < n; i += THREADS) {
-    const uint64_t k = list[i];
+  if (threadIdx.x == 0 && (n & 1)) list[n] = 0;                 // an even number of keys, read two at a time
+  __syncthreads();
+  const ulonglong2* pairs = reinterpret_cast<const ulonglong2*>(list);
+  // four threads count for a key
+  for (int i = threadIdx.x >> 2; i - (int)(threadIdx.x >> 2) < n; i += THREADS / 4) {
+    const uint64_t k = i < n ? list[i] : ~0ull;
     int rank = 0;
-    for (int j = 0; j < n; ++j) rank += list[j] > k;
-    if (rank < K) sc.sorted[rank] = k;
+    for (int j = threadIdx.x & 3; j < (n + 1) / 2; j += 4) {
+      const ulonglong2 two = pairs[j];
+      rank += (two.x > k) + (two.y > k);
+    }
+    rank += __shfl_xor_sync(0xffffffffu, rank, 1);
+    rank += __shfl_xor_sync(0xffffffffu, rank, 2);
+    if ((threadIdx.x & 3) == 0 && i < n && rank < K) sc.sorted[rank] = k;
   }
   __syncthreads();
   return K;
