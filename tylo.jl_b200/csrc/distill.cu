@@ -26,97 +26,170 @@ struct DistillArgs {
 // Places for K entries in each of the three arrays, so that what follows them is 16-byte aligned.
 __host__ __device__ constexpr int entry_slots(int K) { return (K + 3) / 4 * 4; }
 
-// The teacher's probabilities of a row into shared memory (-1 as the index of an entry that is left out); returns the normaliser's
-// logarithm, so that log p_k = v_k / u - the result, and P through `mass`.
-template <int THREADS>
-__device__ __forceinline__ float teacher_row(const DistillArgs& a, size_t row, float* p, int* index, float* scratch, float& mass) {
-  const float* v = a.teacher + row * a.K;
-  const int32_t* id = a.index + row * a.K;
-  float m = -INFINITY;
-  for (int k = threadIdx.x; k < a.K; k += THREADS) {
-    const int j = id[k];
-    const bool live = j >= 0 && j < a.M;
-    const float z = live ? v[k] / a.teacher_temperature : -INFINITY;
-    index[k] = live ? j : -1;
-    p[k] = z;
-    m = fmaxf(m, z);
+// A row's entries in shared memory.
+struct Entries {
+  float *p, *xk;         // value / temperature, then probability; the student's logit
+  int* index;            // -1: left out
+  __device__ __forceinline__ Entries(void* space, int slots)
+      : p(reinterpret_cast<float*>(space)), xk(p + slots), index(reinterpret_cast<int*>(xk + slots)) {}
+};
+
+// Entries `first`, `first + STEP`, ... of a row, four asked for at a time.  The logits are read before any gradient is written (dX may
+// be X).
+template <typename T, int STEP>
+__device__ __forceinline__ void load_entries(const DistillArgs& a, const Entries& e, size_t row, const T* x, int first, int slots) {
+  const float* teacher = a.teacher + row * a.K;
+  const int32_t* ids = a.index + row * a.K;
+  for (int k0 = first; k0 < slots; k0 += 4 * STEP) {
+    int id[4];
+    float value[4], logit[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int k = k0 + i * STEP;
+      id[i] = k < a.K ? ids[k] : -1;
+      value[i] = k < a.K ? teacher[k] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (id[i] >= a.M) id[i] = -1;
+      logit[i] = id[i] >= 0 ? Elem<T>::to_f(x[id[i]]) : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int k = k0 + i * STEP;
+      if (k >= slots) break;
+      e.index[k] = id[i] >= 0 ? id[i] : -1;
+      e.p[k] = id[i] >= 0 ? value[i] / a.teacher_temperature : -INFINITY;
+      e.xk[k] = logit[i];
+    }
   }
-  float log_norm = 0.f;
-  if (a.renormalize) {
-    m = block_reduce<THREADS>(m, MaxOp(), -INFINITY, scratch);
-    const float mo = m == -INFINITY ? 0.f : m;
-    float s = 0.f;
-    for (int k = threadIdx.x; k < a.K; k += THREADS) s += expf(p[k] - mo);
-    s = block_reduce<THREADS>(s, SumOp(), 0.f, scratch);
-    log_norm = s == 0.f ? 0.f : mo + logf(s);
-  }
-  float sum = 0.f;
-  for (int k = threadIdx.x; k < a.K; k += THREADS) {
-    p[k] = expf(p[k] - log_norm);
-    sum += p[k];
-  }
-  mass = block_reduce<THREADS>(sum, SumOp(), 0.f, scratch);     // its barriers also publish p and index
-  return log_norm;
 }
 
-// GROUPS > 0: the part waits in shared memory for the second look.  Dynamic shared memory: the teacher's entries, then the part.
+// By one warp, all lanes: probabilities from values; returns their sum, and the logarithm of the normaliser.
+__device__ __forceinline__ float teacher_probabilities(const DistillArgs& a, const Entries& e, float& log_norm) {
+  const int lane = threadIdx.x & 31;
+  log_norm = 0.f;
+  float sum = 0.f;
+  if (a.renormalize) {
+    float m = -INFINITY;
+    for (int k = lane; k < a.K; k += 32) m = fmaxf(m, e.p[k]);
+    m = warp_max(m);
+    m = m == -INFINITY ? 0.f : m;
+    for (int k = lane; k < a.K; k += 32) sum += expf(e.p[k] - m);
+    sum = warp_reduce(sum, SumOp());
+    log_norm = sum == 0.f ? 0.f : m + logf(sum);
+  }
+  sum = 0.f;
+  for (int k = lane; k < a.K; k += 32) {
+    const float p = expf(e.p[k] - log_norm);
+    e.p[k] = p;
+    sum += p;
+  }
+  return warp_reduce(sum, SumOp());
+}
+
+// Threads beside those that work on the row: where value and gradient are computed together, a warp of its own has the entries ready
+// by the time the sums are (on one of the row's warps, before or after its share of the sums, all others wait for it: 4096 x 32768 bf16
+// with 128 entries 137 and 120 us).
+constexpr int distill_extra(bool loss, bool grad) { return loss && grad ? 32 : 0; }
+constexpr int distill_ctas(int threads, int groups, bool grad) {
+  return groups ? (threads == 128 ? 7 : threads == 256 ? 4 : 2) : 512 / threads * (grad ? 3 : 4);     // (480: 1)
+}
+
+// GROUPS > 0: the part waits in shared memory for the second look.  Dynamic shared memory: the entries, then the part.
 template <typename T, int THREADS, int U, int GROUPS, bool LOSS, bool GRAD>
-__global__ void __launch_bounds__(THREADS, THREADS == 128 ? 8 : THREADS == 256 ? 5 : GROUPS ? 2 : GRAD ? 3 : 4)
+__global__ void __launch_bounds__(THREADS + distill_extra(LOSS, GRAD), distill_ctas(THREADS, GROUPS, GRAD))
 distill_row_kernel(const DistillArgs a, int parts) {
+  constexpr bool EXTRA = distill_extra(LOSS, GRAD) > 0;
   __shared__ float scratch[100];
   extern __shared__ uint4 dynamic[];
   const int slots = entry_slots(a.K);
-  float *p = reinterpret_cast<float*>(dynamic), *xk = p + slots;
-  int* index = reinterpret_cast<int*>(xk + slots);
-  uint4* kept = reinterpret_cast<uint4*>(index + slots);
+  const Entries e(dynamic, slots);
+  uint4* kept = reinterpret_cast<uint4*>(e.index + slots);
   const size_t row = blockIdx.x / parts;
   const T* x = (const T*)a.X + row * a.ldx;
   const VocabRow<T> r(x, a.M);
   const VocabPart part(blockIdx.x % parts, parts, r.whole);
   const float it = 1.f / a.temperature, scale = kVocabLog2e / a.temperature;
-  VocabStats st;
-  if constexpr (GROUPS > 0) st = vocab_resident_stats<T, THREADS, U, GROUPS, false>(kept, x, r, part, scale);
-  else if constexpr (LOSS) st = vocab_thread_stats<T, THREADS, U, false, GRAD, false>(x, r, part, scale, nullptr);
-  float mass;
-  const float log_norm = teacher_row<THREADS>(a, row, p, index, scratch, mass);
-  for (int k = threadIdx.x; k < a.K; k += THREADS) xk[k] = index[k] >= 0 ? Elem<T>::to_f(x[index[k]]) : 0.f;
-  if constexpr (LOSS) vocab_reduce<THREADS, false>(st, scale, scratch, parts);
-  else st = {a.inMx[row], 0.f, a.inL[row], 0.f};
+  const bool on_row = !EXTRA || threadIdx.x < THREADS;
+  const bool on_entries = EXTRA ? threadIdx.x >= THREADS : threadIdx.x < 32;      // a warp
+  const int lane = threadIdx.x & 31;
+  float w = 0.f, log_norm = 0.f;
+  if constexpr (GRAD) w = a.dLoss[row] * it;
+  VocabStats st{-INFINITY, -INFINITY, 0.f, 0.f};
+  if (on_row) {
+    if constexpr (GROUPS > 0) {
+      vocab_resident_ask<T, THREADS, U, GROUPS>(kept, x, r, part);
+      st = vocab_resident_stats<T, THREADS, U, GROUPS, false>(kept, x, r, part, scale);
+    } else if constexpr (LOSS) {
+      st = vocab_thread_stats<T, THREADS, U, false, GRAD, false>(x, r, part, scale, nullptr);
+    } else {
+      st = {a.inMx[row], 0.f, a.inL[row], 0.f};
+    }
+  }
+  auto probabilities = [&]() {
+    const float mass = teacher_probabilities(a, e, log_norm);
+    if (lane == 0) scratch[99] = mass;
+  };
+  if constexpr (EXTRA) {
+    if (on_entries) {
+      load_entries<T, 32>(a, e, row, x, lane, slots);
+      __syncwarp();
+      probabilities();
+    }
+    vocab_reduce<THREADS, false>(st, scale, scratch, parts);      // its barriers publish the entries
+  } else {
+    load_entries<T, THREADS>(a, e, row, x, threadIdx.x, slots);
+    if constexpr (LOSS) vocab_reduce<THREADS, false>(st, scale, scratch, parts);
+    else __syncthreads();
+    if (on_entries && (GRAD || part.part == 0)) probabilities();
+    if constexpr (GRAD) __syncthreads();
+  }
   const float mo = st.m == -INFINITY ? 0.f : st.m;
-  if (LOSS && part.part == 0) {
+  if (LOSS && on_entries && part.part == 0) {
     const float logL = st.s == 0.f ? 0.f : logf(st.s);
+    const float* teacher = a.teacher + row * a.K;
     float loss = 0.f;
-    for (int k = threadIdx.x; k < a.K; k += THREADS)
-      if (index[k] >= 0 && p[k] != 0.f)
-        loss += p[k] * ((a.teacher[row * a.K + k] / a.teacher_temperature - log_norm) - ((xk[k] - mo) / a.temperature - logL));
-    loss = block_reduce<THREADS>(loss, SumOp(), 0.f, scratch);
-    if (threadIdx.x == 0) {
+    for (int k = lane; k < a.K; k += 32) {
+      const float p = e.p[k];
+      if (e.index[k] >= 0 && p != 0.f) loss += p * ((teacher[k] / a.teacher_temperature - log_norm) - ((e.xk[k] - mo) / a.temperature - logL));
+    }
+    loss = warp_reduce(loss, SumOp());
+    if (lane == 0) {
       a.Loss[row] = loss;
       if (a.Mx) { a.Mx[row] = st.m; a.L[row] = st.s; }
     }
   }
   if constexpr (GRAD) {
+    const float mass = scratch[99];
     T* dx = (T*)a.dX + row * a.ldx;
-    const float w = a.dLoss[row] * it;
     if (w == 0.f || mass == 0.f || st.s == 0.f) {       // no weight, no teacher or no probability anywhere
-      vocab_zero<T, THREADS>(dx, r, part);
+      if (on_row) vocab_zero<T, THREADS>(dx, r, part);
     } else {
       const float2 m2 = make_float2(-mo, -mo), sc = make_float2(scale, scale), c = make_float2(w * mass / st.s, w * mass / st.s);
       auto grad = [&](float2 f) {
         const float2 y = __fmul2_rn(__fadd2_rn(f, m2), sc);
         return __fmul2_rn(make_float2(vocab_ex2(y.x), vocab_ex2(y.y)), c);
       };
-      if (!LOSS) __syncthreads();             // xk is read before any gradient is written: dX may be X
-      if constexpr (GROUPS > 0) vocab_resident_rewrite<T, THREADS, U>(dx, kept, x, r, part, grad);
-      else vocab_rewrite<T, THREADS, U>(dx, x, r, part, grad);
+      if (on_row) {
+        if constexpr (GROUPS > 0) vocab_resident_rewrite<T, THREADS, U>(dx, kept, x, r, part, grad);
+        else vocab_rewrite<T, THREADS, U>(dx, x, r, part, grad);
+      }
       __syncthreads();
       // the teacher's entries in this part: every copy of an index sums all its copies in the same order and stores the same value
-      for (int k = threadIdx.x; k < a.K; k += THREADS) {
-        const int j = index[k];
+      const int4* four = reinterpret_cast<const int4*>(e.index);
+      for (int k = threadIdx.x; k < a.K; k += THREADS + distill_extra(LOSS, GRAD)) {
+        const int j = e.index[k];
         if (j < 0 || part.template owner<THREADS>(r, j) < 0) continue;
         float sum = 0.f;
-        for (int i = 0; i < a.K; ++i) sum += index[i] == j ? p[i] : 0.f;
-        dx[j] = Elem<T>::from_f(grad(make_float2(xk[k], 0.f)).x - w * sum);
+        for (int i = 0; i < slots / 4; ++i) {
+          const int4 q = four[i];
+          if (q.x == j) sum += e.p[4 * i];
+          if (q.y == j) sum += e.p[4 * i + 1];
+          if (q.z == j) sum += e.p[4 * i + 2];
+          if (q.w == j) sum += e.p[4 * i + 3];
+        }
+        dx[j] = Elem<T>::from_f(grad(make_float2(e.xk[k], 0.f)).x - w * sum);
       }
     }
   }
@@ -127,21 +200,26 @@ template <typename T, bool LOSS, bool GRAD>
 static int32_t distill_dispatch(const char* who, const DistillArgs& a, int64_t N, cudaStream_t stream) {
   const int64_t packets = a.M / Elem<T>::kVec;
   const int entries = 12 * entry_slots(a.K);
-  if constexpr (!LOSS) {       // nothing to tell one another: plain CTAs, as many per row as fill the GPU several times over
-    int parts = 1;
-    while (parts < 64 && N * parts < 16 * sm_count() && packets >= 8LL * parts * 512) parts *= 2;
+  if constexpr (!LOSS) {
+    // nothing to tell one another: plain CTAs of 4,096 packets, of 1,024 where the rows are few
+    int64_t parts = (packets + 4095) / 4096;
+    if (N * parts < 8 * sm_count()) parts = (packets + 1023) / 1024;
+    parts = parts > 0 ? parts : 1;
     if (packets <= 1024) distill_row_kernel<T, 128, 4, 0, LOSS, GRAD><<<(unsigned)N, 128, entries, stream>>>(a, 1);
-    else distill_row_kernel<T, 512, 4, 0, LOSS, GRAD><<<(unsigned)(N * parts), 512, entries, stream>>>(a, parts);
+    else distill_row_kernel<T, 256, 4, 0, LOSS, GRAD><<<(unsigned)(N * parts), 256, entries, stream>>>(a, (int)parts);
     return check_launch(who);
   } else {
     const int parts = vocab_parts(N, packets);
+    const int64_t per = (packets + parts - 1) / parts;
     if constexpr (!GRAD) {
-      if (packets <= 1024) return launch_vocab(who, distill_row_kernel<T, 128, 4, 0, LOSS, GRAD>, a, N, parts, 128, stream, entries);
-      return launch_vocab(who, distill_row_kernel<T, 512, 4, 0, LOSS, GRAD>, a, N, parts, 512, stream, entries);
+#define TYLO_FWD(THREADS) launch_vocab(who, distill_row_kernel<T, THREADS, 4, 0, LOSS, GRAD>, a, N, parts, THREADS, stream, entries)
+      TYLO_VOCAB_STREAM(TYLO_FWD);
+#undef TYLO_FWD
     } else {
-      const int64_t per = (packets + parts - 1) / parts;
-#define TYLO_BOTH(THREADS, U, GROUPS) \
-  launch_vocab(who, distill_row_kernel<T, THREADS, U, GROUPS, LOSS, GRAD>, a, N, parts, THREADS, stream, entries + (GROUPS ? (int)per * 16 : 0))
+      // (without groups 480 threads: with the entries' warp 512, three times 40 registers)
+#define TYLO_BOTH(THREADS, U, GROUPS)                                                                                                  \
+  launch_vocab(who, distill_row_kernel<T, GROUPS ? THREADS : 480, U, GROUPS, LOSS, GRAD>, a, N, parts, (GROUPS ? THREADS : 480) + 32,  \
+               stream, entries + (GROUPS ? (int)per * 16 : 0))
       TYLO_VOCAB_RESIDENT(TYLO_BOTH);
 #undef TYLO_BOTH
     }

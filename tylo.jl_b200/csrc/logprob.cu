@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(THREADS, logprob_ctas(THREADS, ENTROPY, TOP)) 
   const float scale = kVocabLog2e / a.temperature;
   const bool lead = threadIdx.x == 0 && part.part == 0;
   const int target = lead && a.Logp ? a.targets[row] : -1;       // (first used behind the sums: nothing waits for it here)
-  extern __shared__ ulonglong2 top_space[];
+  extern __shared__ uint64_t top_space[];
   TopScratch<THREADS>& top = *reinterpret_cast<TopScratch<THREADS>*>(top_space);
   const VocabCells<THREADS> cells(TOP ? top.cells : nullptr, part.hi - part.lo, 4 * THREADS);
   VocabStats st = vocab_thread_stats<T, THREADS, 4, ENTROPY, false, TOP>(x, r, part, scale, &cells);
@@ -114,8 +114,10 @@ logprob_fwd_bwd_kernel(const LogprobArgs a, int parts) {
   float g = a.targets ? a.dLogp[row] : 0.f;
   const float h = ENTROPY && a.dEntropy ? a.dEntropy[row] : 0.f;
   VocabStats st;
-  if constexpr (GROUPS > 0) st = vocab_resident_stats<T, THREADS, U, GROUPS, ENTROPY>(kept, x, r, part, scale);
-  else st = vocab_thread_stats<T, THREADS, U, ENTROPY, true, false>(x, r, part, scale, nullptr);
+  if constexpr (GROUPS > 0) {
+    vocab_resident_ask<T, THREADS, U, GROUPS>(kept, x, r, part);
+    st = vocab_resident_stats<T, THREADS, U, GROUPS, ENTROPY>(kept, x, r, part, scale);
+  } else st = vocab_thread_stats<T, THREADS, U, ENTROPY, true, false>(x, r, part, scale, nullptr);
   const bool has = target >= 0 && target < a.M;
   const float xt = has ? Elem<T>::to_f(x[target]) : 0.f;
   g = has ? g : 0.f;
@@ -148,13 +150,13 @@ template <typename T, bool ENTROPY>
 static int32_t logprob_fwd_dispatch(const char* who, const LogprobArgs& a, int64_t N, cudaStream_t stream) {
   const int64_t packets = a.M / Elem<T>::kVec;
   const int parts = vocab_parts(N, packets);
-#define TYLO_FWD(THREADS, TOP) \
-  launch_vocab(who, logprob_fwd_kernel<T, THREADS, ENTROPY, TOP>, a, N, parts, THREADS, stream, TOP ? (int)sizeof(TopScratch<THREADS>) : 0)
   const int64_t per = (packets + parts - 1) / parts;
-  if (a.top) return a.top <= 64 ? TYLO_FWD(256, true) : TYLO_FWD(512, true);
-  if (per <= 2048) return TYLO_FWD(128, false);
-  if (per <= 8192) return TYLO_FWD(256, false);
-  return TYLO_FWD(512, false);
+#define TYLO_TOP(THREADS) \
+  launch_vocab(who, logprob_fwd_kernel<T, THREADS, ENTROPY, true>, a, N, parts, THREADS, stream, (int)sizeof(TopScratch<THREADS>))
+  if (a.top) return a.top <= 64 ? TYLO_TOP(256) : TYLO_TOP(512);
+#undef TYLO_TOP
+#define TYLO_FWD(THREADS) launch_vocab(who, logprob_fwd_kernel<T, THREADS, ENTROPY, false>, a, N, parts, THREADS, stream)
+  TYLO_VOCAB_STREAM(TYLO_FWD);
 #undef TYLO_FWD
 }
 

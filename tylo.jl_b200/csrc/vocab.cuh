@@ -91,6 +91,7 @@ __device__ __forceinline__ float warp_max(float x) {
 template <int THREADS, bool ENTROPY>
 __device__ __forceinline__ void vocab_reduce(VocabStats& st, float scale, float* scratch, int parts) {
   constexpr int WARPS = THREADS / 32;
+  static_assert(WARPS == 4 || (WARPS >= 8 && WARPS <= 16), "the second sum is over 4, 8 or 16 lanes");
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   float m = warp_max(st.m);
   if (lane == 0) scratch[warp] = m;
@@ -103,7 +104,7 @@ __device__ __forceinline__ void vocab_reduce(VocabStats& st, float scale, float*
   s = lane < WARPS ? scratch[32 + lane] : 0.f;
   a = lane < WARPS ? scratch[64 + lane] : 0.f;
 #pragma unroll
-  for (int o = WARPS / 2; o > 0; o >>= 1) {
+  for (int o = WARPS > 8 ? 8 : WARPS / 2; o > 0; o >>= 1) {
     s += __shfl_xor_sync(0xffffffffu, s, o);
     if constexpr (ENTROPY) a += __shfl_xor_sync(0xffffffffu, a, o);
   }
@@ -160,6 +161,18 @@ template <typename T, int U> __device__ __forceinline__ float packets_max(const 
     for (int u = 0; u < U; ++u) m = __hmax2(m, __hmax2(__hmax2(two(p[u].raw.x), two(p[u].raw.y)), __hmax2(two(p[u].raw.z), two(p[u].raw.w))));
     const float r = fmaxf(Elem<T>::to_f(m.x), Elem<T>::to_f(m.y));
     return r == r ? r : -INFINITY;
+  }
+}
+
+// Element j of a packet, j known at run time only.
+template <typename T> __device__ __forceinline__ float packet_element(const Pack<T>& p, int j) {
+  constexpr int LG = sizeof(T) == 2 ? 1 : 0;
+  const uint32_t w = (j >> LG & 2) ? ((j >> LG & 1) ? p.raw.w : p.raw.z) : ((j >> LG & 1) ? p.raw.y : p.raw.x);
+  if constexpr (sizeof(T) == 4) {
+    return __uint_as_float(w);
+  } else {
+    const unsigned short h = (unsigned short)(w >> ((j & 1) * 16));
+    return Elem<T>::to_f(*reinterpret_cast<const T*>(&h));
   }
 }
 
@@ -239,7 +252,11 @@ __device__ __forceinline__ VocabStats vocab_thread_stats(const T* x, const Vocab
   if constexpr (CELLS) {
     float most = -INFINITY;
     for (int c = 0, i = 0; c < cells->cells; ++i, left -= U * THREADS, q += U * THREADS * VEC) {
-      if (left > 0) {
+      if (left > (U - 1) * THREADS) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) load(p[u], u);
+        most = fmaxf(most, sum.take(p, scale));
+      } else if (left > 0) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           if (left > u * THREADS) load(p[u], u);
@@ -281,23 +298,26 @@ __device__ __forceinline__ void wait_copies(int later) {       // until at most 
 #undef TYLO_WAIT_COPIES
   }
 }
-template <typename T, int THREADS, int U, int GROUPS, bool ENTROPY>
-__device__ __forceinline__ VocabStats vocab_resident_stats(uint4* row, const T* x, const VocabRow<T>& r, const VocabPart& part, float scale) {
+template <typename T, int THREADS, int U, int GROUPS>
+__device__ __forceinline__ void vocab_resident_ask(uint4* row, const T* x, const VocabRow<T>& r, const VocabPart& part) {
   static_assert(GROUPS <= 8, "wait_copies");
-  constexpr int VEC = Elem<T>::kVec;
   const int n = part.hi - part.lo - (int)threadIdx.x;          // this thread's packet k * THREADS is there if n > k * THREADS
   const T* q = x + r.index(part.lo + threadIdx.x);
-  uint4* own = row + threadIdx.x;
-  const uint32_t to = (uint32_t)__cvta_generic_to_shared(own);
+  const uint32_t to = (uint32_t)__cvta_generic_to_shared(row + threadIdx.x);
 #pragma unroll
   for (int g = 0; g < GROUPS; ++g) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int k = (g * U + u) * THREADS;
-      if (n > k) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + k * 16), "l"(q + k * VEC) : "memory");
+      if (n > k) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + k * 16), "l"(q + k * Elem<T>::kVec) : "memory");
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
+}
+template <typename T, int THREADS, int U, int GROUPS, bool ENTROPY>
+__device__ __forceinline__ VocabStats vocab_resident_stats(const uint4* row, const T* x, const VocabRow<T>& r, const VocabPart& part, float scale) {
+  const int n = part.hi - part.lo - (int)threadIdx.x;
+  const uint4* own = row + threadIdx.x;
   VocabSum<T, ENTROPY> sum;
   const int one = part.part == 0 ? r.single(threadIdx.x) : -1;
   if (one >= 0) sum.first(Elem<T>::to_f(x[one]), scale);
@@ -411,11 +431,11 @@ __device__ __forceinline__ int vocab_key_index(uint64_t k) { return 0x7fffffff -
 // to shared memory: little more than K elements unless many sit together in few shares or are equal.  Where they do not fit, the bound
 // is raised by counting, and equal elements at the bound are taken in the order of their index.  What is left is thinned by bisection
 // to K and a few, whose rank is counted.
-constexpr int kTopSlack = 32;
+constexpr int kRanked = TYLO_TOP_MAX + 32;       // most elements that are ranked: lists of 32, one more than can be asked for
 
 template <int THREADS> struct TopScratch {
   static constexpr int kSlots = 4 * THREADS;
-  ulonglong2 keys2[kSlots / 2], few2[(TYLO_TOP_MAX + kTopSlack) / 2];
+  uint64_t keys[kSlots], few[kRanked];
   uint64_t sorted[TYLO_TOP_MAX];
   float cells[kCells][THREADS];
   uint32_t mine[THREADS];                 // the threads' largest elements as keys
@@ -446,7 +466,7 @@ template <typename T, int THREADS, int U>
 __device__ __noinline__ int vocab_top(const T* x, const VocabRow<T> r, const VocabPart part, int K, VocabCells<THREADS> cells, bool all,
                                       TopScratch<THREADS>& sc) {
   constexpr int VEC = Elem<T>::kVec, kTopSlots = TopScratch<THREADS>::kSlots;
-  uint64_t *keys = reinterpret_cast<uint64_t*>(sc.keys2), *few = reinterpret_cast<uint64_t*>(sc.few2);
+  uint64_t *keys = sc.keys, *few = sc.few;
   const int elements = (part.hi - part.lo) * VEC + (part.part == 0 ? r.head + r.tail : 0);
   K = min(K, elements);
   BlockCount<THREADS> count{sc.warp, 0};
@@ -488,15 +508,18 @@ __device__ __noinline__ int vocab_top(const T* x, const VocabRow<T> r, const Voc
   __syncthreads();
   uint32_t t = sc.bound, lo, hi;
   const uint32_t top = sc.most;
-  // Hands the elements of the cells whose maximum reaches `from` to f(values, number of values, first index) by the packet: a warp
-  // lists such cells of its threads and deals their packets over its lanes.  f returns false when it has seen enough.
+  // Hands the elements of the cells whose maximum reaches `from` to f(packet, its elements as bits, index of the first) by the packet: a
+  // warp lists such cells of its threads and deals their packets over its lanes.  f returns false when it has seen enough.
   auto visit = [&](uint32_t from, auto f) {
     bool more = true;
     const int one = part.part == 0 ? r.single(threadIdx.x) : -1;
     if (one >= 0) {
+      Pack<T> p;
       float e[VEC];
-      e[0] = Elem<T>::to_f(x[one]);
-      more = f(e, 1, one);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) e[j] = Elem<T>::to_f(x[one]);
+      p.pack(e);
+      more = f(p, 1u, one);
     }
     if (__all_sync(0xffffffffu, mine < from)) return;
     uint16_t* hits = sc.hits[warp];
@@ -523,11 +546,7 @@ __device__ __noinline__ int vocab_top(const T* x, const VocabRow<T> r, const Voc
         }
 #pragma unroll
         for (int u = 0; u < 4; ++u)
-          if (v[u] < part.hi && more) {
-            float e[VEC];
-            p[u].unpack(e);
-            more = f(e, VEC, r.index(v[u]));
-          }
+          if (v[u] < part.hi && more) more = f(p[u], (1u << VEC) - 1, r.index(v[u]));
       }
       __syncwarp();
     }
@@ -535,32 +554,29 @@ __device__ __noinline__ int vocab_top(const T* x, const VocabRow<T> r, const Voc
   // elements above or at a bound into sc.keys; more than kTopSlots: at least that many
   auto collect = [&](uint32_t from) {
     const float low = from <= 1 ? -INFINITY : vocab_unkey(from);
-    visit(from, [&](const float (&e)[VEC], int n, int first) {
+    visit(from, [&](const Pack<T>& p, uint32_t there, int first) {
+      float e[VEC];
+      p.unpack(e);
       uint32_t hit = 0;
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) hit |= (uint32_t)(j < n && !(e[j] < low)) << j;
-      if (!hit) return true;
-#pragma unroll
-      for (int j = 0; j < VEC; ++j)
-        if ((hit >> j & 1) && vocab_key(e[j]) < from) hit &= ~(1u << j);           // NaN, and bounds without a value of their own
-      const int at = atomicAdd(&sc.n, __popc(hit));
-      int k = at;
-#pragma unroll
-      for (int j = 0; j < VEC; ++j)
-        if (hit >> j & 1) {
-          if (k < kTopSlots) keys[k] = vocab_key(e[j], first + j);
-          ++k;
-        }
-      return at < kTopSlots;
+      for (int j = 0; j < VEC; ++j) hit |= (uint32_t)!(e[j] < low) << j;
+      for (hit &= there; hit; hit &= hit - 1) {
+        const int j = __ffs(hit) - 1;
+        const uint64_t k = vocab_key(packet_element(p, j), first + j);
+        if ((uint32_t)(k >> 32) < from) continue;             // NaN, and bounds without a value of their own
+        const int at = atomicAdd(&sc.n, 1);
+        if (at >= kTopSlots) return false;
+        keys[at] = k;
+      }
+      return true;
     });
     __syncthreads();
     return sc.n;
   };
   auto at_least = [&](uint32_t from) {
     int c = 0;
-    visit(from, [&](const float (&e)[VEC], int n, int) {
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) c += j < n && vocab_key(e[j]) >= from;
+    visit(from, [&](const Pack<T>& p, uint32_t there, int) {
+      for (uint32_t b = there; b; b &= b - 1) c += vocab_key(packet_element(p, __ffs(b) - 1)) >= from;
       return true;
     });
     return count(c);
@@ -638,9 +654,9 @@ __device__ __noinline__ int vocab_top(const T* x, const VocabRow<T> r, const Voc
       __syncthreads();
     }
   }
-  // n >= K different keys: thin them, then rank them
+  // n >= K different keys: thin them if they are many, then rank them
   uint64_t* list = keys;
-  if (n > K + kTopSlack) {
+  if (n > kRanked) {
     constexpr int PER = kTopSlots / THREADS;
     uint64_t mine64[PER];
 #pragma unroll
@@ -654,7 +670,7 @@ __device__ __noinline__ int vocab_top(const T* x, const VocabRow<T> r, const Voc
         if (i * THREADS < n) c += __syncthreads_count(mine64[i] >= mid);
       if (c >= K) {
         lo64 = mid;
-        if (c <= K + kTopSlack) break;
+        if (c <= kRanked) break;
       } else {
         hi64 = mid - 1;
       }
@@ -666,20 +682,34 @@ __device__ __noinline__ int vocab_top(const T* x, const VocabRow<T> r, const Voc
     n = sc.m;
     list = few;
   }
-  if (threadIdx.x == 0 && (n & 1)) list[n] = 0;                 // an even number of keys, read two at a time
+  // every warp sorts 32 of them; a key's rank is its place there and the number of larger keys in each of the other sorted lists
+  const int lists = (n + 31) / 32;
+  for (int l = warp; l < lists; l += THREADS / 32) {
+    uint64_t k = l * 32 + lane < n ? list[l * 32 + lane] : 0;
+#pragma unroll
+    for (int size = 2; size <= 32; size *= 2)
+#pragma unroll
+      for (int step = size / 2; step > 0; step /= 2) {
+        const uint64_t other = __shfl_xor_sync(0xffffffffu, k, step);
+        const bool larger = ((lane & step) == 0) == ((lane & size) == 0 || size == 32);      // falling order in the end
+        if ((other > k) == larger) k = other;
+      }
+    list[l * 32 + lane] = k;
+  }
   __syncthreads();
-  const ulonglong2* pairs = reinterpret_cast<const ulonglong2*>(list);
-  // four threads count for a key
-  for (int i = threadIdx.x >> 2; i - (int)(threadIdx.x >> 2) < n; i += THREADS / 4) {
-    const uint64_t k = i < n ? list[i] : ~0ull;
-    int rank = 0;
-    for (int j = threadIdx.x & 3; j < (n + 1) / 2; j += 4) {
-      const ulonglong2 two = pairs[j];
-      rank += (two.x > k) + (two.y > k);
+  for (int l = warp; l < lists; l += THREADS / 32) {
+    const uint64_t k = list[l * 32 + lane];
+    int rank = lane;
+    for (int o = 0; o < lists; ++o) {
+      if (o == l) continue;
+      const uint64_t* other = list + o * 32;
+      int larger = 0;
+#pragma unroll
+      for (int step = 16; step > 0; step /= 2)
+        if (other[larger + step - 1] > k) larger += step;
+      rank += larger + (other[larger] > k);
     }
-    rank += __shfl_xor_sync(0xffffffffu, rank, 1);
-    rank += __shfl_xor_sync(0xffffffffu, rank, 2);
-    if ((threadIdx.x & 3) == 0 && i < n && rank < K) sc.sorted[rank] = k;
+    if (k && rank < K) sc.sorted[rank] = k;
   }
   __syncthreads();
   return K;
@@ -754,6 +784,12 @@ inline int vocab_parts(int64_t N, int64_t packets, int64_t least = 1024) {
   while (parts < 8 && N * parts * 2 <= 2 * sm_count() && packets >= parts * least) parts *= 2;
   return parts;
 }
+
+// Shape of a kernel that looks at its row once, by the packets of a CTA.
+#define TYLO_VOCAB_STREAM(LAUNCH)        \
+  if (per <= 2048) return LAUNCH(128);   \
+  if (per <= 8192) return LAUNCH(256);   \
+  return LAUNCH(512)
 
 // Shape of a kernel that looks at its row twice: rows of up to kResident packets per CTA wait in shared memory.
 constexpr int kResident = 6784;           // 106 KB: two CTAs per SM
