@@ -61,8 +61,11 @@ __device__ __forceinline__ void logprob_part_grad(const LogprobArgs& a, size_t r
   if (target >= 0 && part.template owner<THREADS>(r, target) == (int)threadIdx.x) dx[target] = Elem<T>::from_f(d(make_float2(xt, 0.f)).x + d.at);
 }
 
-// CTAs per SM: registers for as many as the loads need to be hidden behind one another, or as shared memory holds
-constexpr int logprob_ctas(int threads, bool entropy, bool top) { return 512 / threads * (top ? 2 : entropy ? 3 : 4); }
+// CTAs per SM: registers for as many as the loads need to be hidden behind one another.  With alternatives five of 256 threads, three of
+// 512: 2048 x 131072, 20 of them 107 us with five, 111 with six, 115 with four.
+constexpr int logprob_ctas(int threads, bool entropy, bool top) {
+  return top ? (threads == 256 ? 5 : 3) : 512 / threads * (entropy ? 3 : 4);
+}
 
 template <typename T, int THREADS, bool ENTROPY, bool TOP>
 __global__ void __launch_bounds__(THREADS, logprob_ctas(THREADS, ENTROPY, TOP)) logprob_fwd_kernel(const LogprobArgs a, int parts) {
@@ -153,7 +156,7 @@ static int32_t logprob_fwd_dispatch(const char* who, const LogprobArgs& a, int64
   const int64_t per = (packets + parts - 1) / parts;
 #define TYLO_TOP(THREADS) \
   launch_vocab(who, logprob_fwd_kernel<T, THREADS, ENTROPY, true>, a, N, parts, THREADS, stream, (int)sizeof(TopScratch<THREADS>))
-  if (a.top) return a.top <= 64 ? TYLO_TOP(256) : TYLO_TOP(512);
+  if (a.top) return a.top <= 128 ? TYLO_TOP(256) : TYLO_TOP(512);
 #undef TYLO_TOP
 #define TYLO_FWD(THREADS) launch_vocab(who, logprob_fwd_kernel<T, THREADS, ENTROPY, false>, a, N, parts, THREADS, stream)
   TYLO_VOCAB_STREAM(TYLO_FWD);
