@@ -1160,54 +1160,63 @@ def allocate_top_alternatives(X, top: int) -> TopAlternatives:
                            torch.empty(N, top, dtype=torch.int32, device=X.device))
 
 
+# The small calls of these entry points are bound by the host, so their checks hand the addresses on and the stream is asked for
+# without building a stream object (torch.cuda.current_stream alone takes 3 us of a call's 7).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+
+
+def _launch(entry, device: int, *args):
+    """Calls a library entry on the current stream of `device`, which is made the current device for the call if it is not."""
+    if torch.cuda.current_device() == device:
+        rc = entry(*args, _raw_stream(device))
+    else:
+        with torch.cuda.device(device):
+            rc = entry(*args, _raw_stream(device))
+    if rc != 0:
+        _check(rc)
+
+
 def _logits(X):
-    """(M, N, row stride) of a matrix of logits: rows are contiguous and may lie in a wider buffer."""
+    """(M, N, row stride, device) of a matrix of logits: rows are contiguous and may lie in a wider buffer."""
     if X.dim() != 2:
         raise ValueError("expected a matrix of logits (N, M)")
+    device = X.get_device()
+    if device < 0:
+        raise ValueError("libtylo_b200 takes device arrays (there is no CPU path)")
     N, M = X.shape
     sn, sm = X.stride()
-    if N == 1:
-        sn = max(sn, M)
+    if N == 1 and sn < M:
+        sn = M
     if (sm != 1 and M != 1) or sn < M:
         raise ValueError("rows of logits must be contiguous and must not overlap")
-    return M, N, sn
+    return M, N, sn, device
 
 
-def _row_array(name, t, shape, dtype, X):
+def _arg(name, t, shape, dtype, device):
+    """Address of an array that goes with the logits, checked; None stays None."""
     if t is None:
-        return
-    if tuple(t.shape) != shape or t.dtype != dtype:
+        return None
+    if t.shape != shape or t.dtype != dtype:
         raise ValueError(f"{name}: expected {dtype} of shape {shape}, got {t.dtype} of shape {tuple(t.shape)}")
-    if t.device != X.device:
-        raise ValueError(f"{name} is on {t.device}, the logits on {X.device}")
+    if t.get_device() != device:
+        raise ValueError(f"{name} is on {t.device}, the logits are on device {device}")
     if not t.is_contiguous():
         raise ValueError(f"{name}: arrays must be dense")
+    return t.data_ptr()
 
 
 def _logit_grad(X, dX, ld):
-    """The gradient has the rows of the logits: same shape, type, device and distance between rows."""
-    if dX.shape != X.shape or dX.dtype != X.dtype or dX.device != X.device or _logits(dX)[2] != ld and X.shape[0] != 1:
+    """Address of the gradient, which has the rows of the logits: same shape, type, device and distance between rows."""
+    if dX.shape != X.shape or dX.dtype != X.dtype or dX.get_device() != X.get_device() or (_logits(dX)[2] != ld and X.shape[0] != 1):
         raise ValueError("the gradient must have the shape, type, device and row stride of the logits")
+    return dX.data_ptr()
 
 
-class _on:
-    """Makes a tensor's device the current one for a call, so that streams and launches are that device's."""
-
-    __slots__ = ("index", "before")
-
-    def __init__(self, X):
-        self.index = X.device.index
-        if not X.is_cuda:
-            raise ValueError("libtylo_b200 takes device arrays (there is no CPU path)")
-
-    def __enter__(self):
-        self.before = torch.cuda.current_device()
-        if self.before != self.index:
-            torch.cuda.set_device(self.index)
-
-    def __exit__(self, *exc):
-        if self.before != self.index:
-            torch.cuda.set_device(self.before)
+def _checkpoint_args(checkpoints, N, device):
+    if checkpoints is None:
+        return None, None
+    return (_arg("checkpoints.M", checkpoints[0], (N,), torch.float32, device),
+            _arg("checkpoints.L", checkpoints[1], (N,), torch.float32, device))
 
 
 def _like_logits(X, ld):
@@ -1221,27 +1230,16 @@ def token_logprobs_(logp, X, targets, *, temperature=1.0, entropy=None, top: Opt
     where a buffer is given: ``entropy`` (N,) fp32, the largest alternatives ``top`` and the ``checkpoints`` of the backward.
     ``logp`` and ``targets`` may both be None.  X (N, M): rows may lie in a wider buffer.  A target outside [0, M) is padding:
     its log probability is 0.  Among equal logits the lowest index is the first alternative."""
-    pX, pl, pe = primal(X), primal(logp), primal(entropy)
-    M, N, ld = _logits(pX)
-    _row_array("logp", pl, (N,), torch.float32, pX)
-    _row_array("targets", targets, (N,), torch.int32, pX)
-    _row_array("entropy", pe, (N,), torch.float32, pX)
-    K = 0
-    tl = ti = cm = cl = None
+    pX, f32 = primal(X), torch.float32
+    M, N, ld, dev = _logits(pX)
+    rows, K, tl, ti = (N,), 0, None, None
     if top is not None:
-        tl, ti = top
-        K = int(tl.shape[-1])
-        _row_array("top.logp", tl, (N, K), torch.float32, pX)
-        _row_array("top.index", ti, (N, K), torch.int32, pX)
-        if K == 0:
-            tl = ti = None
-    if checkpoints is not None:
-        cm, cl = checkpoints
-        _row_array("checkpoints.M", cm, (N,), torch.float32, pX)
-        _row_array("checkpoints.L", cl, (N,), torch.float32, pX)
-    with _on(pX):
-        _check(_lib.tylo_b200_token_logprobs_fwd(_p(pl), _p(pe), _p(tl), _p(ti), _p(cm), _p(cl), _p(pX), _p(targets), K, M, N, ld,
-                                                 float(temperature), _dtype(pX), _stream()))
+        K = int(top[0].shape[-1])
+        if K:
+            tl, ti = _arg("top.logp", top[0], (N, K), f32, dev), _arg("top.index", top[1], (N, K), torch.int32, dev)
+    cm, cl = _checkpoint_args(checkpoints, N, dev)
+    _launch(_lib.tylo_b200_token_logprobs_fwd, dev, _arg("logp", primal(logp), rows, f32, dev), _arg("entropy", primal(entropy), rows, f32, dev),
+            tl, ti, cm, cl, pX.data_ptr(), _arg("targets", targets, rows, torch.int32, dev), K, M, N, ld, temperature, _dtype(pX))
     return logp
 
 
@@ -1254,30 +1252,19 @@ def token_logprobs(X, targets=None, *, temperature=1.0, entropy=False, top=0, ch
     return out
 
 
-def _logprob_weights(logp, targets, entropy, pX, N):
-    """(dlogp, entropy, d_entropy) of a backward call, checked."""
-    dl = None if logp is None else logp.shadow
-    pe, de = (None, None) if entropy is None else (entropy.primal, entropy.shadow)
-    _row_array("logp's weights", dl, (N,), torch.float32, pX)
-    _row_array("targets", targets, (N,), torch.int32, pX)
-    _row_array("entropy", pe, (N,), torch.float32, pX)
-    _row_array("entropy's weights", de, (N,), torch.float32, pX)
-    return dl, pe, de
-
-
 def grad_token_logprobs_(logp: Optional[Duplicated], X: Duplicated, targets, *, checkpoints, entropy: Optional[Duplicated] = None,
                          temperature=1.0):
     """Overwrites ``X.shadow`` with the gradient of sum(logp * logp.shadow) + sum(entropy * entropy.shadow); ``entropy.primal`` and
     ``checkpoints`` are the forward's.  ``X.shadow`` has X's row stride and may be X itself."""
-    pX = X.primal
-    M, N, ld = _logits(pX)
-    dl, pe, de = _logprob_weights(logp, targets, entropy, pX, N)
-    _logit_grad(pX, X.shadow, ld)
-    _row_array("checkpoints.M", checkpoints.M, (N,), torch.float32, pX)
-    _row_array("checkpoints.L", checkpoints.L, (N,), torch.float32, pX)
-    with _on(pX):
-        _check(_lib.tylo_b200_token_logprobs_bwd(_p(X.shadow), _p(dl), _p(de), _p(pX), _p(targets), _p(pe), _p(checkpoints.M),
-                                                 _p(checkpoints.L), M, N, ld, float(temperature), _dtype(pX), _stream()))
+    pX, f32 = X.primal, torch.float32
+    M, N, ld, dev = _logits(pX)
+    rows = (N,)
+    H, dH = (None, None) if entropy is None else (entropy.primal, entropy.shadow)
+    cm, cl = _checkpoint_args(checkpoints, N, dev)
+    _launch(_lib.tylo_b200_token_logprobs_bwd, dev, _logit_grad(pX, X.shadow, ld),
+            None if logp is None else _arg("logp's weights", logp.shadow, rows, f32, dev), _arg("entropy's weights", dH, rows, f32, dev),
+            pX.data_ptr(), _arg("targets", targets, rows, torch.int32, dev), _arg("entropy", H, rows, f32, dev), cm, cl, M, N, ld,
+            temperature, _dtype(pX))
 
 
 def grad_token_logprobs(dlogp, X, targets, *, checkpoints, entropy=None, d_entropy=None, temperature=1.0):
@@ -1291,24 +1278,22 @@ def grad_token_logprobs(dlogp, X, targets, *, checkpoints, entropy=None, d_entro
 def token_logprobs_with_grad_(logp: Optional[Duplicated], X: Duplicated, targets, *, entropy: Optional[Duplicated] = None, temperature=1.0):
     """``token_logprobs_`` and ``grad_token_logprobs_`` in one launch, for weights (``logp.shadow``, ``entropy.shadow``) that are known
     before the forward, as in next-token training.  Writes ``logp.primal``, ``entropy.primal`` and ``X.shadow`` (which may be X)."""
-    pX = X.primal
-    M, N, ld = _logits(pX)
-    dl, pe, de = _logprob_weights(logp, targets, entropy, pX, N)
-    pl = None if logp is None else logp.primal
-    _row_array("logp", pl, (N,), torch.float32, pX)
-    _logit_grad(pX, X.shadow, ld)
-    with _on(pX):
-        _check(_lib.tylo_b200_token_logprobs_fwd_bwd(_p(pl), _p(pe), _p(X.shadow), _p(dl), _p(de), _p(pX), _p(targets), M, N, ld,
-                                                     float(temperature), _dtype(pX), _stream()))
+    pX, f32 = X.primal, torch.float32
+    M, N, ld, dev = _logits(pX)
+    rows = (N,)
+    lp, dlp = (None, None) if logp is None else (logp.primal, logp.shadow)
+    H, dH = (None, None) if entropy is None else (entropy.primal, entropy.shadow)
+    _launch(_lib.tylo_b200_token_logprobs_fwd_bwd, dev, _arg("logp", lp, rows, f32, dev), _arg("entropy", H, rows, f32, dev),
+            _logit_grad(pX, X.shadow, ld), _arg("logp's weights", dlp, rows, f32, dev), _arg("entropy's weights", dH, rows, f32, dev),
+            pX.data_ptr(), _arg("targets", targets, rows, torch.int32, dev), M, N, ld, temperature, _dtype(pX))
 
 
-def _distill_args(X, teacher, index, temperature, teacher_temperature, renormalize):
-    M, N, ld = _logits(X)
-    K = int(teacher.shape[-1])
-    _row_array("teacher", teacher, (N, K), torch.float32, X)
-    _row_array("index", index, (N, K), torch.int32, X)
+def _teacher_args(X, teacher, index, temperature, teacher_temperature, renormalize):
+    M, N, ld, dev = _logits(X)
+    shape = (N, int(teacher.shape[-1]))
     u = temperature if teacher_temperature is None else teacher_temperature
-    return N, ld, K, (K, M, N, ld, float(temperature), float(u), int(bool(renormalize)), _dtype(X))
+    return N, ld, dev, (_arg("teacher", teacher, shape, torch.float32, dev), _arg("index", index, shape, torch.int32, dev)), (
+        shape[1], M, N, ld, temperature, u, 1 if renormalize else 0, _dtype(X))
 
 
 def distill_(loss, X, teacher, index, *, temperature=1.0, teacher_temperature=None, renormalize=True, checkpoints=None):
@@ -1317,16 +1302,10 @@ def distill_(loss, X, teacher, index, *, temperature=1.0, teacher_temperature=No
     teacher / teacher_temperature over the row's entries, otherwise its exponential as it is.  ``teacher_temperature`` defaults to
     ``temperature``; the alternatives of ``token_logprobs_`` already have theirs in them, so they go with 1.  Entries with an
     index outside [0, M) are left out."""
-    pX, pl = primal(X), primal(loss)
-    N, ld, K, args = _distill_args(pX, teacher, index, temperature, teacher_temperature, renormalize)
-    _row_array("loss", pl, (N,), torch.float32, pX)
-    cm = cl = None
-    if checkpoints is not None:
-        cm, cl = checkpoints
-        _row_array("checkpoints.M", cm, (N,), torch.float32, pX)
-        _row_array("checkpoints.L", cl, (N,), torch.float32, pX)
-    with _on(pX):
-        _check(_lib.tylo_b200_distill_fwd(_p(pl), _p(cm), _p(cl), _p(pX), _p(teacher), _p(index), *args, _stream()))
+    pX = primal(X)
+    N, ld, dev, entries, how = _teacher_args(pX, teacher, index, temperature, teacher_temperature, renormalize)
+    cm, cl = _checkpoint_args(checkpoints, N, dev)
+    _launch(_lib.tylo_b200_distill_fwd, dev, _arg("loss", primal(loss), (N,), torch.float32, dev), cm, cl, pX.data_ptr(), *entries, *how)
     return loss
 
 
@@ -1341,14 +1320,10 @@ def grad_distill_(loss: Duplicated, X: Duplicated, teacher, index, *, checkpoint
     """Overwrites ``X.shadow`` with the gradient of sum(loss * loss.shadow); ``checkpoints`` are the forward's.  ``X.shadow`` has
     X's row stride and may be X itself.  The teacher's entries are constants."""
     pX = X.primal
-    N, ld, K, args = _distill_args(pX, teacher, index, temperature, teacher_temperature, renormalize)
-    _row_array("the loss's weights", loss.shadow, (N,), torch.float32, pX)
-    _logit_grad(pX, X.shadow, ld)
-    _row_array("checkpoints.M", checkpoints.M, (N,), torch.float32, pX)
-    _row_array("checkpoints.L", checkpoints.L, (N,), torch.float32, pX)
-    with _on(pX):
-        _check(_lib.tylo_b200_distill_bwd(_p(X.shadow), _p(loss.shadow), _p(pX), _p(teacher), _p(index), _p(checkpoints.M),
-                                          _p(checkpoints.L), *args, _stream()))
+    N, ld, dev, entries, how = _teacher_args(pX, teacher, index, temperature, teacher_temperature, renormalize)
+    cm, cl = _checkpoint_args(checkpoints, N, dev)
+    _launch(_lib.tylo_b200_distill_bwd, dev, _logit_grad(pX, X.shadow, ld), _arg("the loss's weights", loss.shadow, (N,), torch.float32, dev),
+            pX.data_ptr(), *entries, cm, cl, *how)
 
 
 def grad_distill(dloss, X, teacher, index, *, checkpoints, **kw):
@@ -1361,14 +1336,10 @@ def grad_distill(dloss, X, teacher, index, *, checkpoints, **kw):
 def distill_with_grad_(loss: Duplicated, X: Duplicated, teacher, index, *, temperature=1.0, teacher_temperature=None, renormalize=True):
     """``distill_`` and ``grad_distill_`` in one launch, for weights (``loss.shadow``) that are known before the forward.  Writes
     ``loss.primal`` and ``X.shadow`` (which may be X)."""
-    pX = X.primal
-    N, ld, K, args = _distill_args(pX, teacher, index, temperature, teacher_temperature, renormalize)
-    _row_array("loss", loss.primal, (N,), torch.float32, pX)
-    _row_array("the loss's weights", loss.shadow, (N,), torch.float32, pX)
-    _logit_grad(pX, X.shadow, ld)
-    with _on(pX):
-        _check(_lib.tylo_b200_distill_fwd_bwd(_p(loss.primal), _p(X.shadow), _p(loss.shadow), _p(pX), _p(teacher), _p(index), *args,
-                                              _stream()))
+    pX, f32 = X.primal, torch.float32
+    N, ld, dev, entries, how = _teacher_args(pX, teacher, index, temperature, teacher_temperature, renormalize)
+    _launch(_lib.tylo_b200_distill_fwd_bwd, dev, _arg("loss", loss.primal, (N,), f32, dev), _logit_grad(pX, X.shadow, ld),
+            _arg("the loss's weights", loss.shadow, (N,), f32, dev), pX.data_ptr(), *entries, *how)
 
 
 # ---------------------------------------------------------------------------------------------
