@@ -404,7 +404,8 @@ int32_t tylo_b200_softmax_bwd(void* dX, const void* dY, const void* Y, int64_t M
  *  - Masked logits may be -Inf or the lowest value of the type.  A row of nothing but -Inf has no probability anywhere: its
  *    statistics are (-Inf, 0), its log probabilities -Inf, its entropy 0, its gradient zero.  A NaN or +Inf makes its row NaN.
  *  - Token ids are 0-based int32.  An id outside [0, M) stands for "no token" (padding).
- *  - dX has the rows of X (same M, N, ldx) and may be the same memory as X.  A row whose weights are all zero gets zeros.
+ *  - dX has the rows of X (same M, N, ldx); it is X itself or does not overlap it.  No other result may overlap an argument.  A row
+ *    whose weights are all zero gets zeros.
  *  - Results do not depend on the order in which the GPU works: equal inputs give equal bits. */
 #define TYLO_TOP_MAX 256       /* most alternatives per row */
 #define TYLO_DISTILL_MAX 1024  /* most teacher entries per row */

@@ -63,6 +63,24 @@ def test_distillation(tylo):
     assert lib.tylo_b200_distill_fwd_bwd(f(1), ctypes.c_void_p(0x1008), f(7), f(2), f(3), f(4), 8, 64, 4, 64, 1.0, 1.0, 1, 0, None) == 3
 
 
+def test_overlapping_arrays_are_refused(tylo):
+    lib = tylo._lib
+    err = lib.tylo_b200_last_error
+    at = ctypes.c_void_p
+    # 4 rows of 64 fp32 logits, 256 elements apart: the gradient shifted by 16 bytes, by a row, into the gap (the check behind it fails)
+    bwd = lambda dX, M=64, ld=256, N=4, dt=0: lib.tylo_b200_token_logprobs_bwd(at(dX), f(2), None, at(0x100000), f(4), None, None, None, M, N, ld, 1.0, dt, None)
+    for dX in (0x100010, 0x100000 - 16, 0x100000 + 4 * 256, 0x100000 - 4 * 256, 0x100000 + 4 * 60, 0x100000 + 4 * (3 * 256 + 60)):
+        assert bwd(dX) == 1 and b"overlap" in err()
+    for dX in (0x100000, 0x100000 + 4 * 64, 0x100000 + 4 * 192, 0x100000 + 4 * (3 * 256 + 64), 0x100000 - 4 * (3 * 256 + 64)):
+        assert bwd(dX) == 1 and b"checkpoints" in err()
+    assert bwd(0x100000 + 2 * 64, dt=1) == 1 and b"checkpoints" in err()
+    assert bwd(0x100000 + 2 * 56, dt=1) == 1 and b"overlap" in err()
+    w = f(9)
+    assert lib.tylo_b200_token_logprobs_fwd_bwd(w, None, f(2), w, None, f(3), f(4), 64, 4, 64, 1.0, 0, None) == 1 and b"different" in err()
+    assert lib.tylo_b200_distill_fwd_bwd(w, f(2), w, f(3), f(4), f(5), 8, 64, 4, 64, 1.0, 1.0, 1, 0, None) == 1 and b"different" in err()
+    assert lib.tylo_b200_distill_bwd(at(0x3010), w, f(3), f(4), f(5), f(6), f(7), 8, 64, 4, 64, 1.0, 1.0, 1, 0, None) == 1 and b"overlap" in err()
+
+
 def test_host_arrays_are_refused(tylo):
     import torch
     X, t, w = torch.zeros(4, 64), torch.zeros(4, dtype=torch.int32), torch.zeros(4)

@@ -30,6 +30,9 @@ def logits(rng, N, M, dt, *, pad=0, kind="normal"):
         x[N // 2] = 0.0
     elif kind == "rising":          # every element beats all before it
         x = np.broadcast_to(np.linspace(-60, 60, M), (N, M)).copy()
+    elif kind == "stripes":         # what is large sits in the shares of few threads: packets 0 to 59 of every 256
+        vec = 4 if dt == "f32" else 8
+        x += np.where(np.arange(M) // vec % 256 < 60, 30.0, 0.0)
     elif kind == "large":           # far from zero: only differences matter
         x = x + 3e4 if dt == "f16" else x + 1e6
     buf = torch.full((N, M + pad), 7.0, dtype=TORCH_DT[dt], device="cuda")
@@ -77,8 +80,9 @@ def test_scores(tylo, oracle, N, M, dt):
 
 
 @pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("kind", ["masked", "lowest", "ties", "rising", "large"])
-@pytest.mark.parametrize("N,M,K,tau", [(5, 300, 256, 1.0), (3, 5000, 256, 0.6), (4, 33001, 64, 2.0), (200, 20011, 100, 1.0), (2, 200000, 256, 1.0)])
+@pytest.mark.parametrize("kind", ["masked", "lowest", "ties", "rising", "stripes", "large"])
+@pytest.mark.parametrize("N,M,K,tau", [(5, 300, 256, 1.0), (3, 5000, 256, 0.6), (4, 33001, 64, 2.0), (200, 20011, 100, 1.0), (300, 40000, 64, 1.0),
+                                       (300, 10000, 256, 1.0), (2, 200000, 256, 1.0)])
 def test_scores_of_odd_rows(tylo, oracle, N, M, K, tau, kind, dt):
     rng = np.random.default_rng(M + K)
     X, X64, _ = logits(rng, N, M, dt, kind=kind, pad=3)

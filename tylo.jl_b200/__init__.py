@@ -1239,7 +1239,7 @@ def token_logprobs_(logp, X, targets, *, temperature=1.0, entropy=None, top: Opt
             tl, ti = _arg("top.logp", top[0], (N, K), f32, dev), _arg("top.index", top[1], (N, K), torch.int32, dev)
     cm, cl = _checkpoint_args(checkpoints, N, dev)
     _launch(_lib.tylo_b200_token_logprobs_fwd, dev, _arg("logp", primal(logp), rows, f32, dev), _arg("entropy", primal(entropy), rows, f32, dev),
-            tl, ti, cm, cl, pX.data_ptr(), _arg("targets", targets, rows, torch.int32, dev), K, M, N, ld, temperature, _dtype(pX))
+            tl, ti, cm, cl, pX.data_ptr(), _arg("targets", targets, rows, torch.int32, dev), K, M, N, ld, float(temperature), _dtype(pX))
     return logp
 
 
@@ -1264,7 +1264,7 @@ def grad_token_logprobs_(logp: Optional[Duplicated], X: Duplicated, targets, *, 
     _launch(_lib.tylo_b200_token_logprobs_bwd, dev, _logit_grad(pX, X.shadow, ld),
             None if logp is None else _arg("logp's weights", logp.shadow, rows, f32, dev), _arg("entropy's weights", dH, rows, f32, dev),
             pX.data_ptr(), _arg("targets", targets, rows, torch.int32, dev), _arg("entropy", H, rows, f32, dev), cm, cl, M, N, ld,
-            temperature, _dtype(pX))
+            float(temperature), _dtype(pX))
 
 
 def grad_token_logprobs(dlogp, X, targets, *, checkpoints, entropy=None, d_entropy=None, temperature=1.0):
@@ -1285,7 +1285,7 @@ def token_logprobs_with_grad_(logp: Optional[Duplicated], X: Duplicated, targets
     H, dH = (None, None) if entropy is None else (entropy.primal, entropy.shadow)
     _launch(_lib.tylo_b200_token_logprobs_fwd_bwd, dev, _arg("logp", lp, rows, f32, dev), _arg("entropy", H, rows, f32, dev),
             _logit_grad(pX, X.shadow, ld), _arg("logp's weights", dlp, rows, f32, dev), _arg("entropy's weights", dH, rows, f32, dev),
-            pX.data_ptr(), _arg("targets", targets, rows, torch.int32, dev), M, N, ld, temperature, _dtype(pX))
+            pX.data_ptr(), _arg("targets", targets, rows, torch.int32, dev), M, N, ld, float(temperature), _dtype(pX))
 
 
 def _teacher_args(X, teacher, index, temperature, teacher_temperature, renormalize):
@@ -1293,7 +1293,7 @@ def _teacher_args(X, teacher, index, temperature, teacher_temperature, renormali
     shape = (N, int(teacher.shape[-1]))
     u = temperature if teacher_temperature is None else teacher_temperature
     return N, ld, dev, (_arg("teacher", teacher, shape, torch.float32, dev), _arg("index", index, shape, torch.int32, dev)), (
-        shape[1], M, N, ld, temperature, u, 1 if renormalize else 0, _dtype(X))
+        shape[1], M, N, ld, float(temperature), float(u), 1 if renormalize else 0, _dtype(X))
 
 
 def distill_(loss, X, teacher, index, *, temperature=1.0, teacher_temperature=None, renormalize=True, checkpoints=None):

@@ -6,6 +6,11 @@
 //   dX_j = w / t (P q_j - sum_{k: I_k = j} p_k),   P = sum_k p_k
 //
 // Entries with an index outside [0, M) are left out, of the teacher's normalisation too.
+//
+// Bound and shapes as in logprob.cu; the entries come on top: 64 of them cost the forward nothing that shows (4096 x 65536 bf16 87 us), 128
+// cost value and gradient of 4096 x 32768 15 us of 107, of 4096 x 131072 25 of 425, and the backward of 4096 x 32768 12 of 97.  The entries
+// of a row are dealt with by one warp, so their sums are the same for every shape; an index that occurs more than once is summed in
+// the order of the entries by whoever stores it, so no order of the GPU's shows.
 #include "vocab.cuh"
 
 namespace tylo {
@@ -65,27 +70,28 @@ __device__ __forceinline__ void load_entries(const DistillArgs& a, const Entries
   }
 }
 
-// By one warp, all lanes: probabilities from values; returns their sum, and the logarithm of the normaliser.
-__device__ __forceinline__ float teacher_probabilities(const DistillArgs& a, const Entries& e, float& log_norm) {
+// By one warp, all lanes: probabilities exp(z_k - m) / S from values z_k; returns their sum, and m and log S.
+__device__ __forceinline__ float teacher_probabilities(const DistillArgs& a, const Entries& e, float& m, float& log_sum) {
   const int lane = threadIdx.x & 31;
-  log_norm = 0.f;
-  float sum = 0.f;
+  m = log_sum = 0.f;
   if (a.renormalize) {
-    float m = -INFINITY;
-    for (int k = lane; k < a.K; k += 32) m = fmaxf(m, e.p[k]);
-    m = warp_max(m);
-    m = m == -INFINITY ? 0.f : m;
-    for (int k = lane; k < a.K; k += 32) sum += expf(e.p[k] - m);
-    sum = warp_reduce(sum, SumOp());
-    log_norm = sum == 0.f ? 0.f : m + logf(sum);
+    float most = -INFINITY;
+    for (int k = lane; k < a.K; k += 32) most = fmaxf(most, e.p[k]);
+    most = warp_max(most);
+    m = most == -INFINITY ? 0.f : most;
   }
-  sum = 0.f;
+  float sum = 0.f;
   for (int k = lane; k < a.K; k += 32) {
-    const float p = expf(e.p[k] - log_norm);
+    const float p = expf(e.p[k] - m);
     e.p[k] = p;
     sum += p;
   }
-  return warp_reduce(sum, SumOp());
+  sum = warp_reduce(sum, SumOp());
+  if (!a.renormalize || sum == 0.f) return sum;
+  log_sum = logf(sum);
+  const float inv = 1.f / sum;
+  for (int k = lane; k < a.K; k += 32) e.p[k] *= inv;
+  return sum * inv;
 }
 
 // Threads beside those that work on the row: where value and gradient are computed together, a warp of its own has the entries ready
@@ -114,7 +120,7 @@ distill_row_kernel(const DistillArgs a, int parts) {
   const bool on_row = !EXTRA || threadIdx.x < THREADS;
   const bool on_entries = EXTRA ? threadIdx.x >= THREADS : threadIdx.x < 32;      // a warp
   const int lane = threadIdx.x & 31;
-  float w = 0.f, log_norm = 0.f;
+  float w = 0.f, teacher_max = 0.f, teacher_log = 0.f;
   if constexpr (GRAD) w = a.dLoss[row] * it;
   VocabStats st{-INFINITY, -INFINITY, 0.f, 0.f};
   if (on_row) {
@@ -128,7 +134,7 @@ distill_row_kernel(const DistillArgs a, int parts) {
     }
   }
   auto probabilities = [&]() {
-    const float mass = teacher_probabilities(a, e, log_norm);
+    const float mass = teacher_probabilities(a, e, teacher_max, teacher_log);
     if (lane == 0) scratch[99] = mass;
   };
   if constexpr (EXTRA) {
@@ -152,7 +158,7 @@ distill_row_kernel(const DistillArgs a, int parts) {
     float loss = 0.f;
     for (int k = lane; k < a.K; k += 32) {
       const float p = e.p[k];
-      if (e.index[k] >= 0 && p != 0.f) loss += p * ((teacher[k] / a.teacher_temperature - log_norm) - ((e.xk[k] - mo) / a.temperature - logL));
+      if (e.index[k] >= 0 && p != 0.f) loss += p * ((teacher[k] / a.teacher_temperature - teacher_max - teacher_log) - ((e.xk[k] - mo) / a.temperature - logL));
     }
     loss = warp_reduce(loss, SumOp());
     if (lane == 0) {
@@ -209,7 +215,7 @@ static int32_t distill_dispatch(const char* who, const DistillArgs& a, int64_t N
     else distill_row_kernel<T, 256, 4, 0, LOSS, GRAD><<<(unsigned)(N * parts), 256, entries, stream>>>(a, (int)parts);
     return check_launch(who);
   } else {
-    const int parts = vocab_parts(N, packets);
+    const int parts = GRAD ? vocab_parts_twice(N, packets, 20480) : vocab_parts(N, packets);
     const int64_t per = (packets + parts - 1) / parts;
     if constexpr (!GRAD) {
 #define TYLO_FWD(THREADS) launch_vocab(who, distill_row_kernel<T, THREADS, 4, 0, LOSS, GRAD>, a, N, parts, THREADS, stream, entries)
@@ -267,8 +273,8 @@ extern "C" int32_t tylo_b200_distill_bwd(void* dX, const float* dLoss, const voi
                                          tylo_stream_t stream) {
   const char* who = "distill_bwd";
   if (int32_t rc = check_distill(who, X, teacher, index, K, M, N, ldx, temperature, teacher_temperature)) return rc;
-  TYLO_REQUIRE(dX && dLoss, TYLO_ERR_INVALID_ARGUMENT, "%s: dX and dLoss must be non-null", who);
-  TYLO_REQUIRE(aligned16(dX), TYLO_ERR_MISALIGNED, "%s: dX must be 16-byte aligned", who);
+  if (int32_t rc = check_vocab_grad(who, dX, X, M, N, ldx, dtype)) return rc;
+  TYLO_REQUIRE(dLoss, TYLO_ERR_INVALID_ARGUMENT, "%s: dLoss must be non-null", who);
   TYLO_REQUIRE(Mx && L, TYLO_ERR_INVALID_ARGUMENT, "%s: checkpoints Mx and L from the forward are required", who);
   DistillArgs a = distill_args(X, teacher, index, K, M, ldx, temperature, teacher_temperature, renormalize);
   a.dX = dX; a.dLoss = dLoss; a.inMx = Mx; a.inL = L;
@@ -281,8 +287,9 @@ extern "C" int32_t tylo_b200_distill_fwd_bwd(float* Loss, void* dX, const float*
                                              float teacher_temperature, int32_t renormalize, int32_t dtype, tylo_stream_t stream) {
   const char* who = "distill_fwd_bwd";
   if (int32_t rc = check_distill(who, X, teacher, index, K, M, N, ldx, temperature, teacher_temperature)) return rc;
-  TYLO_REQUIRE(Loss && dX && dLoss, TYLO_ERR_INVALID_ARGUMENT, "%s: Loss, dX and dLoss must be non-null", who);
-  TYLO_REQUIRE(aligned16(dX), TYLO_ERR_MISALIGNED, "%s: dX must be 16-byte aligned", who);
+  if (int32_t rc = check_vocab_grad(who, dX, X, M, N, ldx, dtype)) return rc;
+  TYLO_REQUIRE(Loss && dLoss, TYLO_ERR_INVALID_ARGUMENT, "%s: Loss and dLoss must be non-null", who);
+  TYLO_REQUIRE(Loss != dLoss, TYLO_ERR_INVALID_ARGUMENT, "%s: Loss and dLoss must be different arrays", who);
   DistillArgs a = distill_args(X, teacher, index, K, M, ldx, temperature, teacher_temperature, renormalize);
   a.Loss = Loss; a.dX = dX; a.dLoss = dLoss;
   TYLO_DISPATCH_DTYPE(dtype, T, return (distill_dispatch<T, true, true>(who, a, N, (cudaStream_t)stream)));

@@ -2,6 +2,15 @@
 //
 //   logp = y_target - log L,   H = log L - A / L,   A = sum exp(y) y                      (y, L as in vocab.cuh)
 //   dX_j = 1/t ( g ([j = target] - p_j) - h p_j (log p_j + H) )
+//
+// Forward: one pass over the row, which memory bounds: 2048 x 131072 bf16 in 85 us = 6.3 TB/s (a plain read of the same bytes takes 76),
+// 4096 x 131072 in 159 us = 6.8 TB/s; the special-function units, one exponential per logit, are three quarters busy beside it.  Smaller
+// CTAs for shorter rows, so that starting a CTA and joining its sums weigh less: 4096 x 32768 50 us with 256 threads, 8192 x 16000 50 us
+// with 128 and 67 with 512.  With 20 alternatives 109 us for 2048 x 131072 and 78 for 4096 x 32768, with 128 of them 128 and 101: what
+// follows the sums is a chain of short steps, hidden only by the other CTAs of the SM.
+// Backward: one read and one write, 4096 x 65536 bf16 159 us = 6.8 TB/s, with the entropy's weight 161 us.
+// Value and gradient in one launch read the logits from memory once: 4096 x 32768 bf16 91 us = 5.9 TB/s (98 us under the power cap of a
+// longer run) against 135 for the two calls, 2048 x 131072 196 us (the second look finds two thirds of a longer row in L2).
 #include "vocab.cuh"
 
 namespace tylo {
@@ -31,7 +40,7 @@ template <bool ENTROPY> struct LogprobGrad {
   float2 mo, scale, A, B;
   float at;
   __device__ __forceinline__ LogprobGrad(float mx, float L, float g, float h, float H, float temperature) {
-    const float it = 1.f / temperature, c = it / L, m = mx == -INFINITY ? 0.f : -mx, k = kVocabLog2e * it;
+    const float it = 1.f / temperature, c = it / L, m = mx == -INFINITY ? 0.f : -mx, k = kVocabLog2e / temperature;
     // -p (g + h (log p + H)) / t with log p = ln 2 (y - log2 L)
     const float a = -h * kVocabLn2 * c, b = -(ENTROPY ? g + h * (H - logf(L)) : g) * c;
     mo = make_float2(m, m); scale = make_float2(k, k); A = make_float2(a, a); B = make_float2(b, b);
@@ -45,7 +54,7 @@ template <bool ENTROPY> struct LogprobGrad {
   }
 };
 
-// The gradient of a part, which waits in `kept` or is read (again).  `xt`: the target's logit, read before anything is written (dX may
+// The gradient of a part, which waits in `kept` or, without that, is read (again).  `xt`: the target's logit, read before anything is written (dX may
 // be X); target < 0: none.  A row without weights or without any probability gets zeros.
 template <typename T, int THREADS, int U, bool ENTROPY>
 __device__ __forceinline__ void logprob_part_grad(const LogprobArgs& a, size_t row, const T* x, const uint4* kept, const VocabRow<T>& r,
@@ -101,8 +110,8 @@ __global__ void __launch_bounds__(THREADS, logprob_ctas(THREADS, ENTROPY, TOP)) 
   cluster_done(parts);
 }
 
-// Value and gradient.  GROUPS > 0: the part waits in shared memory for the second look; 0: it is read again, out of L2 as far as it is
-// still there.
+// Value and gradient.  GROUPS > 0: the part waits in shared memory for the second look (4096 x 32768 bf16 91 us; read again from L2 it
+// took 105); 0: it is too long for that and is read again, out of L2 as far as it is still there.
 template <typename T, int THREADS, int U, int GROUPS, bool ENTROPY>
 __global__ void __launch_bounds__(THREADS, THREADS == 128 ? 8 : THREADS == 256 ? 5 : GROUPS ? 2 : 3)
 logprob_fwd_bwd_kernel(const LogprobArgs a, int parts) {
@@ -135,6 +144,8 @@ logprob_fwd_bwd_kernel(const LogprobArgs a, int parts) {
   cluster_done(parts);
 }
 
+// 2,048 packets per CTA: a row's coefficients cost a thread as much as three packets (1,024: 4096 x 65536 bf16 with both weights 200 us,
+// 161 with 2,048).
 template <typename T, int THREADS, bool ENTROPY>
 __global__ void __launch_bounds__(THREADS, 6) logprob_bwd_kernel(const LogprobArgs a, int parts) {
   const size_t row = blockIdx.x / parts;
@@ -154,6 +165,8 @@ static int32_t logprob_fwd_dispatch(const char* who, const LogprobArgs& a, int64
   const int64_t packets = a.M / Elem<T>::kVec;
   const int parts = vocab_parts(N, packets);
   const int64_t per = (packets + parts - 1) / parts;
+  // 256 threads up to 128 alternatives (4096 x 32768 bf16, 128 of them: 101 us, with 512 threads 143); more would be half of the threads and
+  // above, whose maxima bound next to nothing
 #define TYLO_TOP(THREADS) \
   launch_vocab(who, logprob_fwd_kernel<T, THREADS, ENTROPY, true>, a, N, parts, THREADS, stream, (int)sizeof(TopScratch<THREADS>))
   if (a.top) return a.top <= 128 ? TYLO_TOP(256) : TYLO_TOP(512);
@@ -166,7 +179,7 @@ static int32_t logprob_fwd_dispatch(const char* who, const LogprobArgs& a, int64
 template <typename T, bool ENTROPY>
 static int32_t logprob_fwd_bwd_dispatch(const char* who, const LogprobArgs& a, int64_t N, cudaStream_t stream) {
   const int64_t packets = a.M / Elem<T>::kVec;
-  const int parts = vocab_parts(N, packets);
+  const int parts = vocab_parts_twice(N, packets, 14336);
   const int64_t per = (packets + parts - 1) / parts;
 #define TYLO_BOTH(THREADS, U, GROUPS) \
   launch_vocab(who, logprob_fwd_bwd_kernel<T, THREADS, U, GROUPS, ENTROPY>, a, N, parts, THREADS, stream, GROUPS ? (int)per * 16 : 0)
@@ -208,9 +221,7 @@ extern "C" int32_t tylo_b200_token_logprobs_fwd(float* Logp, float* Entropy, flo
   return TYLO_OK;
 }
 
-static int32_t check_logprob_grad(const char* who, const void* dX, const float* dLogp, const float* dEntropy, const int32_t* targets) {
-  TYLO_REQUIRE(dX, TYLO_ERR_INVALID_ARGUMENT, "%s: dX must be non-null", who);
-  TYLO_REQUIRE(aligned16(dX), TYLO_ERR_MISALIGNED, "%s: dX must be 16-byte aligned", who);
+static int32_t check_logprob_weights(const char* who, const float* dLogp, const float* dEntropy, const int32_t* targets) {
   TYLO_REQUIRE(!dLogp == !targets, TYLO_ERR_INVALID_ARGUMENT, "%s: dLogp and targets go together", who);
   TYLO_REQUIRE(dLogp || dEntropy, TYLO_ERR_INVALID_ARGUMENT, "%s: dLogp or dEntropy is required", who);
   return TYLO_OK;
@@ -222,7 +233,8 @@ extern "C" int32_t tylo_b200_token_logprobs_bwd(void* dX, const float* dLogp, co
                                                 tylo_stream_t stream) {
   const char* who = "token_logprobs_bwd";
   if (int32_t rc = check_vocab(who, X, M, N, ldx, temperature)) return rc;
-  if (int32_t rc = check_logprob_grad(who, dX, dLogp, dEntropy, targets)) return rc;
+  if (int32_t rc = check_vocab_grad(who, dX, X, M, N, ldx, dtype)) return rc;
+  if (int32_t rc = check_logprob_weights(who, dLogp, dEntropy, targets)) return rc;
   TYLO_REQUIRE(Mx && L, TYLO_ERR_INVALID_ARGUMENT, "%s: checkpoints Mx and L from the forward are required", who);
   TYLO_REQUIRE(!dEntropy || Entropy, TYLO_ERR_INVALID_ARGUMENT, "%s: dEntropy needs the forward's Entropy", who);
   LogprobArgs a = {};
@@ -237,8 +249,11 @@ extern "C" int32_t tylo_b200_token_logprobs_fwd_bwd(float* Logp, float* Entropy,
                                                     float temperature, int32_t dtype, tylo_stream_t stream) {
   const char* who = "token_logprobs_fwd_bwd";
   if (int32_t rc = check_vocab(who, X, M, N, ldx, temperature)) return rc;
-  if (int32_t rc = check_logprob_grad(who, dX, dLogp, dEntropy, targets)) return rc;
+  if (int32_t rc = check_vocab_grad(who, dX, X, M, N, ldx, dtype)) return rc;
+  if (int32_t rc = check_logprob_weights(who, dLogp, dEntropy, targets)) return rc;
   TYLO_REQUIRE(!Logp || targets, TYLO_ERR_INVALID_ARGUMENT, "%s: Logp needs targets", who);
+  TYLO_REQUIRE((!Logp || Logp != dLogp) && (!Entropy || Entropy != dEntropy), TYLO_ERR_INVALID_ARGUMENT,
+               "%s: results and their weights must be different arrays", who);
   LogprobArgs a = {};
   a.X = X; a.targets = targets; a.Logp = Logp; a.Entropy = Entropy; a.dX = dX; a.dLogp = dLogp; a.dEntropy = dEntropy;
   a.ldx = ldx; a.M = (int)M; a.temperature = temperature;

@@ -3,7 +3,7 @@
 //   y_j = (x_j - max x) / t,  L = sum exp(y_j),  p_j = exp(y_j) / L,  entropy = log L - sum exp(y_j) y_j / L
 //
 // Differences are taken before the scale: the lowest finite value overflows with a factor above 1, and a logit of a thousand
-// would lose ten bits of its difference.  Both terms of the entropy are positive, so nothing cancels.
+// would lose ten bits of its difference.  Both terms of the entropy are positive, so it does not cancel.
 // Exponents are in units of log 2; the smallest that is used as a factor is kExpFloor, whose exp2 is zero: an entry of -Inf
 // adds 0 * kExpFloor = 0 where 0 * -Inf would be NaN.  The sum itself takes the exponent as it is, so a NaN or +Inf reaches it.
 // A row made only of -Inf has L = 0 and no probability anywhere.
@@ -51,10 +51,16 @@ __device__ __forceinline__ uint4 ld_logits(const void* p) {
   return v;
 }
 
-// The same for rows that are read twice: they stay in L2 before what is read or written once.
+// The same with a place in L2: a row that will be read again stays there before what is read or written once (4096 x 131072 bf16, value
+// and gradient 414 us, 454 without), and is the first to go when it has been.
 __device__ __forceinline__ uint64_t keep_policy() {
   uint64_t p;
   asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(p));
+  return p;
+}
+__device__ __forceinline__ uint64_t drop_policy() {
+  uint64_t p;
+  asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
   return p;
 }
 __device__ __forceinline__ uint4 ld_logits(const void* p, uint64_t policy) {
@@ -66,7 +72,8 @@ __device__ __forceinline__ uint4 ld_logits(const void* p, uint64_t policy) {
 
 // Running statistics of a row or of a part of it: largest logit, the reference that the exponentials are taken against, sum of
 // e = exp2((x - ref) * scale), sum of e times its exponent.  The reference follows the maximum only when that is more than
-// kRefSlack (in units of log 2) above it: sums in floating point are as good, and the branch that rescales them stays rare.
+// kRefSlack (in units of log 2) above it: sums in floating point are as good (the entropy's second sum to kRefSlack * 2^-24), and the
+// branch that rescales them stays rare (2048 x 131072 bf16 92 and 89 us).
 constexpr float kRefSlack = 8.f;
 
 struct VocabStats {
@@ -337,6 +344,10 @@ __device__ __forceinline__ VocabStats vocab_resident_stats(const uint4* row, con
   return sum.stats();
 }
 
+// Special-function units: a fourth of the exponentials as polynomials on the multiply-add pipes was slower everywhere (entropy 169 and
+// 181 us, value and gradient 91 and 93), and so was one fused multiply-add per exponent against a rounded reference (no change): what is
+// left is memory and, in longer runs, the power cap (1000 W, 1.76 GHz).
+
 // Gradient of a part that waits in shared memory (vocab_resident_stats): f(pair of logits) -> pair of gradients for every element,
 // rounded once, on the way out.
 template <typename T, int THREADS, int U, typename F>
@@ -379,6 +390,7 @@ __device__ __forceinline__ void vocab_rewrite(T* dx, const T* x, const VocabRow<
     p.pack(e);
     st_stream(to, p.raw);
   };
+  const uint64_t drop = drop_policy();
   const int n = part.hi - part.lo, steps = n / (U * THREADS);
   const int first = r.index(part.lo + threadIdx.x);
   {
@@ -386,7 +398,7 @@ __device__ __forceinline__ void vocab_rewrite(T* dx, const T* x, const VocabRow<
     Pack<T> p[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (left > u * THREADS) p[u].raw = ld_logits(x + i + u * (THREADS * VEC));
+      if (left > u * THREADS) p[u].raw = ld_logits(x + i + u * (THREADS * VEC), drop);
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (left > u * THREADS) give(p[u], dx + i + u * (THREADS * VEC));
@@ -396,7 +408,7 @@ __device__ __forceinline__ void vocab_rewrite(T* dx, const T* x, const VocabRow<
     T* to = dx + first + k * (U * THREADS * VEC);
     Pack<T> p[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) p[u].raw = ld_logits(q + u * (THREADS * VEC));
+    for (int u = 0; u < U; ++u) p[u].raw = ld_logits(q + u * (THREADS * VEC), drop);
 #pragma unroll
     for (int u = 0; u < U; ++u) give(p[u], to + u * (THREADS * VEC));
   }
@@ -786,10 +798,17 @@ int32_t launch_vocab(const char* who, void (*kernel)(A, int), const A& args, int
 }
 
 // CTAs per row: a row is dealt over a cluster while rows alone leave SMs without a CTA.
-inline int vocab_parts(int64_t N, int64_t packets, int64_t least = 1024) {
+inline int vocab_parts(int64_t N, int64_t packets) {
   int parts = 1;
-  while (parts < 8 && N * parts * 2 <= 2 * sm_count() && packets >= parts * least) parts *= 2;
+  while (parts < 8 && N * parts * 2 <= 2 * sm_count() && packets >= parts * 1024LL) parts *= 2;
   return parts;
+}
+// The same for kernels that look at their row twice: rows longer than `pair` packets go to two CTAs, so that fewer of them are under way
+// and the second look finds more in L2.  Value and gradient, bf16, us with one CTA / two: log probabilities 2048 x 100,000 157 / 165,
+// 2048 x 131,072 213 / 193, 2048 x 262,144 458 / 420; distillation 4096 x 131,072 425 / 433, 2048 x 200,000 359 / 329.
+inline int vocab_parts_twice(int64_t N, int64_t packets, int64_t pair) {
+  const int parts = vocab_parts(N, packets);
+  return packets > pair && parts < 2 ? 2 : parts;
 }
 
 // Shape of a kernel that looks at its row once, by the packets of a CTA.
@@ -798,7 +817,8 @@ inline int vocab_parts(int64_t N, int64_t packets, int64_t least = 1024) {
   if (per <= 8192) return LAUNCH(256);   \
   return LAUNCH(512)
 
-// Shape of a kernel that looks at its row twice: rows of up to kResident packets per CTA wait in shared memory.
+// Shape of a kernel that looks at its row twice: rows of up to kResident packets per CTA wait in shared memory.  Value and gradient, bf16, us,
+// waiting / read again: 8192 x 16000 81 / 90, 4096 x 32768 83 / 93, 2048 x 50000 75 / 77.
 constexpr int kResident = 6784;           // 106 KB: two CTAs per SM
 #define TYLO_VOCAB_RESIDENT(LAUNCH)                                      \
   if (per <= 1024) return LAUNCH(128, 4, 2);                             \
@@ -806,6 +826,17 @@ constexpr int kResident = 6784;           // 106 KB: two CTAs per SM
   if (per <= 4096) return LAUNCH(256, 4, 4);                             \
   if (per <= kResident) return LAUNCH(512, 2, 7);                        \
   return LAUNCH(512, 4, 0)
+
+// The gradient of N rows of M logits, rows ldx apart, is written over the logits themselves or anywhere beside them.
+inline int32_t check_vocab_grad(const char* who, const void* dX, const void* X, int64_t M, int64_t N, int64_t ldx, int32_t dtype) {
+  TYLO_REQUIRE(dX, TYLO_ERR_INVALID_ARGUMENT, "%s: dX must be non-null", who);
+  TYLO_REQUIRE(aligned16(dX), TYLO_ERR_MISALIGNED, "%s: dX must be 16-byte aligned", who);
+  const int64_t apart = ((const char*)dX - (const char*)X) / (dtype == TYLO_F32 ? 4 : 2), within = (apart % ldx + ldx) % ldx;
+  const bool far = apart >= (N - 1) * ldx + M || -apart >= (N - 1) * ldx + M;
+  TYLO_REQUIRE(apart == 0 || far || (within >= M && ldx - within >= M), TYLO_ERR_INVALID_ARGUMENT,
+               "%s: dX must be X or not overlap it", who);
+  return TYLO_OK;
+}
 
 inline int32_t check_vocab(const char* who, const void* X, int64_t M, int64_t N, int64_t ldx, float temperature) {
   TYLO_REQUIRE(X, TYLO_ERR_INVALID_ARGUMENT, "%s: X must be non-null", who);
