@@ -73,7 +73,7 @@ __device__ __forceinline__ void logprob_part_grad(const LogprobArgs& a, size_t r
 // CTAs per SM: registers for as many as the loads need to be hidden behind one another.  With alternatives five of 256 threads, three of
 // 512: 2048 x 131072, 20 of them 107 us with five, 111 with six, 115 with four.
 constexpr int logprob_ctas(int threads, bool entropy, bool top) {
-  return top ? (threads == 256 ? 5 : 3) : 512 / threads * (entropy ? 3 : 4);
+  return top ? (threads == 128 ? 8 : threads == 256 ? 5 : 3) : 512 / threads * (entropy ? 3 : 4);
 }
 
 template <typename T, int THREADS, bool ENTROPY, bool TOP>
@@ -166,9 +166,11 @@ static int32_t logprob_fwd_dispatch(const char* who, const LogprobArgs& a, int64
   const int parts = vocab_parts(N, packets);
   const int64_t per = (packets + parts - 1) / parts;
   // 256 threads up to 128 alternatives (4096 x 32768 bf16, 128 of them: 101 us, with 512 threads 143); more would be half of the threads and
-  // above, whose maxima bound next to nothing
+  // above, whose maxima bound next to nothing.  128 threads for many short rows (20 of them, 256 / 128 threads: 8192 x 16000 108 / 81 us,
+  // 4096 x 32768 78 / 71, 2048 x 131072 with 64 of them 115 / 123, 256 x 32000 13.2 / 15.6)
 #define TYLO_TOP(THREADS) \
   launch_vocab(who, logprob_fwd_kernel<T, THREADS, ENTROPY, true>, a, N, parts, THREADS, stream, (int)sizeof(TopScratch<THREADS>))
+  if (a.top && a.top <= 64 && per <= 4096 && N * parts >= 8 * sm_count()) return TYLO_TOP(128);
   if (a.top) return a.top <= 128 ? TYLO_TOP(256) : TYLO_TOP(512);
 #undef TYLO_TOP
 #define TYLO_FWD(THREADS) launch_vocab(who, logprob_fwd_kernel<T, THREADS, ENTROPY, false>, a, N, parts, THREADS, stream)
