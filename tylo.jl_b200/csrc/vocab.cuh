@@ -451,7 +451,7 @@ template <int THREADS> struct TopScratch {
   uint64_t sorted[TYLO_TOP_MAX];
   float cells[kCells][THREADS];
   uint32_t mine[THREADS];                 // the threads' largest elements as keys
-  uint32_t warp[64], bound, most;
+  uint32_t warp[64], bound, most, dense;
   uint16_t hits[THREADS / 32][64];
   int rank[TYLO_TOP_MAX];
   int n, m;
@@ -486,7 +486,7 @@ __device__ __noinline__ int vocab_top(const T* x, const VocabRow<T> r, const Voc
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint32_t mine = sc.mine[threadIdx.x];
   if (warp == 0) {
-    // one warp looks for the bound, by bisection between the smallest and the largest maximum; an eighth more than K will do
+    // one warp looks for the bound, by bisection between the smallest and the largest maximum; a few more than K will do
     uint32_t k[THREADS / 32], hi = 0, lo = 0xffffffffu;
     int live = 0;
 #pragma unroll
@@ -499,7 +499,8 @@ __device__ __noinline__ int vocab_top(const T* x, const VocabRow<T> r, const Voc
     hi = __reduce_max_sync(0xffffffffu, hi);
     lo = __reduce_min_sync(0xffffffffu, lo) + 1;
     const uint32_t most = hi;
-    if (__reduce_add_sync(0xffffffffu, live) >= K) {
+    int reach = __reduce_add_sync(0xffffffffu, live);
+    if (reach >= K) {
       while (lo < hi) {
         const uint32_t mid = lo + (hi - lo) / 2 + 1;
         int c = 0;
@@ -508,7 +509,8 @@ __device__ __noinline__ int vocab_top(const T* x, const VocabRow<T> r, const Voc
         c = __reduce_add_sync(0xffffffffu, c);
         if (c >= K) {
           lo = mid;
-          if (c <= K + K / 8) break;
+          reach = c;
+          if (c <= K + K / 32 + 2) break;
         } else {
           hi = mid - 1;
         }
@@ -516,7 +518,8 @@ __device__ __noinline__ int vocab_top(const T* x, const VocabRow<T> r, const Voc
     } else {
       lo = 1;                               // below every element
     }
-    if (lane == 0) { sc.bound = lo; sc.most = most; sc.n = 0; sc.m = 0; }
+    // (many maxima equal to the bound, as where a mask leaves little: its equals would not fit, so they are not tried)
+    if (lane == 0) { sc.bound = lo; sc.most = most; sc.dense = lo > 1 && reach >= 2 * K + 32; sc.n = 0; sc.m = 0; }
   }
   __syncthreads();
   uint32_t t = sc.bound, lo, hi;
@@ -534,14 +537,16 @@ __device__ __noinline__ int vocab_top(const T* x, const VocabRow<T> r, const Voc
       p.pack(e);
       more = f(p, 1u, one);
     }
-    if (__all_sync(0xffffffffu, mine < from)) return;
+    const bool any = mine >= from;
+    if (!__any_sync(0xffffffffu, any)) return;
+    const float low = from <= 1 ? -INFINITY : vocab_unkey(from);       // (without a value of its own it is a NaN: `all` alone counts)
     uint16_t* hits = sc.hits[warp];
     static_assert(U == 4, "packets of a cell as a power of two");
     const int lg = cells.shift + 2, per = 1 << lg;
     for (int c = 0; c < cells.cells;) {
       int n = 0;
       for (; c < cells.cells && n <= 32; ++c) {
-        const bool hit = mine >= from && (all || vocab_key(cells.max[c][threadIdx.x]) >= from);
+        const bool hit = any && (all || cells.max[c][threadIdx.x] >= low);
         const uint32_t mask = __ballot_sync(0xffffffffu, hit);
         if (hit) hits[n + __popc(mask & ((1u << lane) - 1))] = (uint16_t)(c * 32 + lane);
         n += __popc(mask);
@@ -600,7 +605,7 @@ __device__ __noinline__ int vocab_top(const T* x, const VocabRow<T> r, const Voc
     __syncthreads();
   };
   auto above = [&](uint32_t bound) { return bound == 0xffffffffu ? 0 : collect(bound + 1); };     // nothing is above a NaN
-  int n = collect(t);
+  int n = sc.dense ? kTopSlots + 1 : collect(t);
   if (n > kTopSlots) {
     clear();
     n = above(t);
