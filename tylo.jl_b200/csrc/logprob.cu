@@ -6,8 +6,8 @@
 // Forward: one pass over the row, which memory bounds: 2048 x 131072 bf16 in 85 us = 6.3 TB/s (a plain read of the same bytes takes 76),
 // 4096 x 131072 in 159 us = 6.8 TB/s; the special-function units, one exponential per logit, are three quarters busy beside it.  Smaller
 // CTAs for shorter rows, so that starting a CTA and joining its sums weigh less: 4096 x 32768 50 us with 256 threads, 8192 x 16000 50 us
-// with 128 and 67 with 512.  With 20 alternatives 109 us for 2048 x 131072 and 78 for 4096 x 32768, with 128 of them 128 and 101: what
-// follows the sums is a chain of short steps, hidden only by the other CTAs of the SM.
+// with 128 and 67 with 512.  With 20 alternatives 104 us for 2048 x 131072 and 69 for 4096 x 32768, with 128 of them 122 and 96: what
+// follows the sums is a chain of short steps (without it the same kernel takes 88 and 54), hidden by the other CTAs of the SM only.
 // Backward: one read and one write, 4096 x 65536 bf16 159 us = 6.8 TB/s, with the entropy's weight 161 us.
 // Value and gradient in one launch read the logits from memory once: 4096 x 32768 bf16 91 us = 5.9 TB/s (98 us under the power cap of a
 // longer run) against 135 for the two calls, 2048 x 131072 196 us (the second look finds two thirds of a longer row in L2).
@@ -165,13 +165,14 @@ static int32_t logprob_fwd_dispatch(const char* who, const LogprobArgs& a, int64
   const int64_t packets = a.M / Elem<T>::kVec;
   const int parts = vocab_parts(N, packets);
   const int64_t per = (packets + parts - 1) / parts;
-  // 256 threads up to 128 alternatives (4096 x 32768 bf16, 128 of them: 101 us, with 512 threads 143); more would be half of the threads and
-  // above, whose maxima bound next to nothing.  128 threads for many short rows (20 of them, 256 / 128 threads: 8192 x 16000 108 / 81 us,
-  // 4096 x 32768 78 / 71, 2048 x 131072 with 64 of them 115 / 123, 256 x 32000 13.2 / 15.6)
+  // us, bf16.  256 threads up to 176 alternatives (256 / 512 threads: 4096 x 32768 with 144 of them 105 / 132, with 200 136 / 143; 2048 x
+  // 131072 129 / 133 and 147 / 142): with more, the threads' maxima bound too little.  128 for a clustered row, whose lists have to fit
+  // into 4 * THREADS places.  128 threads for many short rows (256 / 128: 8192 x 16000 with 20 108 / 81, 4096 x 32768 78 / 71, 2048 x 131072
+  // with 64 115 / 123, 256 x 32000 13.2 / 15.6).
 #define TYLO_TOP(THREADS) \
   launch_vocab(who, logprob_fwd_kernel<T, THREADS, ENTROPY, true>, a, N, parts, THREADS, stream, (int)sizeof(TopScratch<THREADS>))
   if (a.top && a.top <= 64 && per <= 4096 && N * parts >= 8 * sm_count()) return TYLO_TOP(128);
-  if (a.top) return a.top <= 128 ? TYLO_TOP(256) : TYLO_TOP(512);
+  if (a.top) return a.top <= (parts == 1 ? 176 : 128) ? TYLO_TOP(256) : TYLO_TOP(512);
 #undef TYLO_TOP
 #define TYLO_FWD(THREADS) launch_vocab(who, logprob_fwd_kernel<T, THREADS, ENTROPY, false>, a, N, parts, THREADS, stream)
   TYLO_VOCAB_STREAM(TYLO_FWD);

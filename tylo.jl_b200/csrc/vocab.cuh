@@ -747,7 +747,7 @@ __device__ __forceinline__ void vocab_ranked(TopScratch<THREADS>& sc, int n, int
   const int me = cluster.block_rank();
   for (int i = n + threadIdx.x; i < K; i += THREADS) sc.sorted[i] = 0;
   cluster.sync();
-  uint64_t* all = sc.keys;                       // parts * K of at most 4 * THREADS places
+  uint64_t* all = sc.keys;                       // parts * K of its 4 * THREADS places (the launch sees to it)
   for (int i = threadIdx.x; i < parts * K; i += THREADS) all[i] = cluster.map_shared_rank(&sc, i / K)->sorted[i % K];
   for (int i = threadIdx.x; i < K; i += THREADS) sc.rank[i] = i;
   __syncthreads();
