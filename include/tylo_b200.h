@@ -406,7 +406,8 @@ int32_t tylo_b200_softmax_bwd(void* dX, const void* dY, const void* Y, int64_t M
  *  - Token ids are 0-based int32.  An id outside [0, M) stands for "no token" (padding).
  *  - dX has the rows of X (same M, N, ldx); it is X itself or does not overlap it.  No other result may overlap an argument.  A row
  *    whose weights are all zero gets zeros.
- *  - Results do not depend on the order in which the GPU works: equal inputs give equal bits. */
+ *  - Results do not depend on the order in which the GPU works: equal calls give equal bits.  (A row's last bits may depend on the
+ *    number of rows it comes with: a batch that leaves SMs idle deals a row over several of them.) */
 #define TYLO_TOP_MAX 256       /* most alternatives per row */
 #define TYLO_DISTILL_MAX 1024  /* most teacher entries per row */
 

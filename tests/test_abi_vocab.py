@@ -19,7 +19,7 @@ def _fwd(lib, Logp=f(1), Entropy=None, TopLogp=None, TopIndex=None, Mx=None, L=N
     (dict(Logp=None, Entropy=f(5)), 1, b"targets"), (dict(Mx=f(4)), 1, b"together"), (dict(top=1), 1, b"TopLogp"), (dict(TopLogp=f(4), TopIndex=f(5)), 1, b"top"),
     (dict(top=-1), 1, b"top"), (dict(top=65, TopLogp=f(4), TopIndex=f(5)), 1, b"at most M"),
     (dict(top=257, M=512, ld=512, TopLogp=f(4), TopIndex=f(5)), 1, b"256"), (dict(dtype=3), 1, b"dtype"), (dict(dtype=9), 1, b"dtype"),
-    (dict(M=1 << 31, ld=1 << 31), 2, b"not supported"), (dict(N=1 << 30), 2, b"not supported")])
+    (dict(M=1 << 31, ld=1 << 31), 2, b"not supported"), (dict(N=1 << 30), 2, b"not supported"), (dict(ld=(1 << 34) + 1), 2, b"not supported")])
 def test_scores(tylo, change, status, word):
     assert _fwd(tylo._lib, **change) == status
     assert word in tylo._lib.tylo_b200_last_error()

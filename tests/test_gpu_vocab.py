@@ -174,6 +174,9 @@ def teacher_entries(rng, N, M, K, kind):
     elif kind == "masked":
         v[rng.random((N, K)) < 0.4] = -np.inf
         v[0] = -np.inf
+    elif kind == "lowest":                           # entries of the lowest value; a row of nothing else is uniform
+        v[rng.random((N, K)) < 0.4] = np.finfo(np.float32).min
+        v[0] = np.finfo(np.float32).min
     return v.astype(np.float32).astype(np.float64), index.astype(np.int32)
 
 
@@ -227,6 +230,47 @@ def test_distillation(tylo, oracle, N, M, K, pad, kind, xkind, renormalize, dt):
     same.copy_(X)
     tylo.grad_distill_(tylo.Duplicated(loss, W), tylo.Duplicated(same, same), V, I, checkpoints=cp, **how)
     assert torch.equal(same, dX), "backward in place"
+
+
+@pytest.mark.parametrize("renormalize", [True, False])
+def test_teacher_of_the_lowest_value(tylo, oracle, renormalize):
+    """A temperature below 1 must not turn the lowest value into -Inf before the largest is taken off."""
+    rng = np.random.default_rng(1)
+    X, X64, _ = logits(rng, 5, 2000, "f32")
+    v, index = teacher_entries(rng, 5, 2000, 40, "lowest")
+    how = dict(temperature=1.0, teacher_temperature=0.25, renormalize=renormalize)
+    loss, dX = torch.empty(5, device="cuda"), like(X)
+    tylo.distill_with_grad_(tylo.Duplicated(loss, dev(np.ones(5))), tylo.Duplicated(X, dX), dev(v), dev(index, torch.int32), **how)
+    # 40 terms of order 10 at 2^-20 each; gradients below 1
+    np.testing.assert_allclose(back(loss), oracle.distill_ref(X64, v, index, 1.0, 0.25, renormalize), rtol=2.0 ** -18, atol=1e-4)
+    np.testing.assert_allclose(back(dX), oracle.distill_bwd_ref(np.ones(5), X64, v, index, 1.0, 0.25, renormalize), rtol=2.0 ** -16, atol=2e-6)
+
+
+def test_the_longest_row(tylo):
+    """One row of 2^31 - 2^16 - 1 logits: indices up to the end of 32 bits.  The reference adds its chunks in 64 bits."""
+    M, piece = (1 << 31) - (1 << 16) - 1, 1 << 26
+    X = torch.empty(1, M, dtype=torch.float16, device="cuda")
+    g = torch.Generator("cuda").manual_seed(2)
+    for at in range(0, M, piece):
+        n = min(piece, M - at)
+        X[0, at:at + n] = torch.randn(n, generator=g, device="cuda", dtype=torch.float16)
+    marks = torch.tensor([M - 1, 0, 12345, M // 2 + 1, M - 5, 1 << 30], device="cuda")
+    X[0, marks] = torch.tensor([20.0, 19.0, 18.0, 18.0, 17.0, 16.0], dtype=torch.float16, device="cuda")
+    total = sum(torch.exp(X[0, at:at + piece].double() - 20.0).sum() for at in range(0, M, piece))
+    target = torch.tensor([M - 5], dtype=torch.int32, device="cuda")
+    got = tylo.token_logprobs(X, target, top=6)
+    assert got.top.index.tolist() == [[M - 1, 0, 12345, M // 2 + 1, M - 5, 1 << 30]]
+    # the sum's chains have 2^18 terms (8 CTAs, 512 threads, 2 each): roundings of up to 2^-24 of the sum add up to about 2^9 of them
+    # at random, 2^-15; 2^-10 leaves 32 times that
+    lse = float(torch.log(total)) + 20.0
+    assert abs(float(got.logp) - (17.0 - lse)) < 2.0 ** -10
+    w = torch.full((1,), 1024.0, device="cuda")
+    lp = torch.empty(1, device="cuda")
+    before = X[0, marks].double()
+    tylo.token_logprobs_with_grad_(tylo.Duplicated(lp, w), tylo.Duplicated(X, X), target)
+    ref = -1024.0 * torch.exp(before - lse)
+    ref[4] += 1024.0
+    assert torch.allclose(X[0, marks].double(), ref, rtol=2.0 ** -9, atol=2.0 ** -20)
 
 
 def test_gradients_against_differences(tylo):

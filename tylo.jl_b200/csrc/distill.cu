@@ -33,7 +33,7 @@ __host__ __device__ constexpr int entry_slots(int K) { return (K + 3) / 4 * 4; }
 
 // A row's entries in shared memory.
 struct Entries {
-  float *p, *xk;         // value / temperature, then probability; the student's logit
+  float *p, *xk;         // the teacher's value, then its probability; the student's logit
   int* index;            // -1: left out
   __device__ __forceinline__ Entries(void* space, int slots)
       : p(reinterpret_cast<float*>(space)), xk(p + slots), index(reinterpret_cast<int*>(xk + slots)) {}
@@ -64,13 +64,14 @@ __device__ __forceinline__ void load_entries(const DistillArgs& a, const Entries
       const int k = k0 + i * STEP;
       if (k >= slots) break;
       e.index[k] = id[i] >= 0 ? id[i] : -1;
-      e.p[k] = id[i] >= 0 ? value[i] / a.teacher_temperature : -INFINITY;
+      e.p[k] = id[i] >= 0 ? value[i] : -INFINITY;
       e.xk[k] = logit[i];
     }
   }
 }
 
-// By one warp, all lanes: probabilities exp(z_k - m) / S from values z_k; returns their sum, and m and log S.
+// By one warp, all lanes: probabilities exp((v_k - m) / u) / S from values v_k (the difference first: the lowest value overflows where it
+// is divided by less than 1); returns their sum, and m and log S.
 __device__ __forceinline__ float teacher_probabilities(const DistillArgs& a, const Entries& e, float& m, float& log_sum) {
   const int lane = threadIdx.x & 31;
   m = log_sum = 0.f;
@@ -82,7 +83,7 @@ __device__ __forceinline__ float teacher_probabilities(const DistillArgs& a, con
   }
   float sum = 0.f;
   for (int k = lane; k < a.K; k += 32) {
-    const float p = expf(e.p[k] - m);
+    const float p = expf((e.p[k] - m) / a.teacher_temperature);
     e.p[k] = p;
     sum += p;
   }
@@ -158,7 +159,7 @@ distill_row_kernel(const DistillArgs a, int parts) {
     float loss = 0.f;
     for (int k = lane; k < a.K; k += 32) {
       const float p = e.p[k];
-      if (e.index[k] >= 0 && p != 0.f) loss += p * ((teacher[k] / a.teacher_temperature - teacher_max - teacher_log) - ((e.xk[k] - mo) / a.temperature - logL));
+      if (e.index[k] >= 0 && p != 0.f) loss += p * (((teacher[k] - teacher_max) / a.teacher_temperature - teacher_log) - ((e.xk[k] - mo) / a.temperature - logL));
     }
     loss = warp_reduce(loss, SumOp());
     if (lane == 0) {

@@ -848,7 +848,8 @@ inline int32_t check_vocab(const char* who, const void* X, int64_t M, int64_t N,
   TYLO_REQUIRE(M > 0 && N > 0, TYLO_ERR_INVALID_ARGUMENT, "%s: extents must be positive (M=%lld, N=%lld)", who, (long long)M,
                (long long)N);
   TYLO_REQUIRE(ldx >= M, TYLO_ERR_INVALID_ARGUMENT, "%s: ldx (%lld) must be at least M (%lld)", who, (long long)ldx, (long long)M);
-  TYLO_REQUIRE(M < 0x7fff0000LL && N <= 0x0fffffffLL, TYLO_ERR_UNSUPPORTED, "%s: M above 2^31-2^16 or N above 2^28-1 is not supported", who);
+  TYLO_REQUIRE(M < 0x7fff0000LL && N <= 0x0fffffffLL && ldx <= 1LL << 34, TYLO_ERR_UNSUPPORTED,
+               "%s: M from 2^31-2^16, N above 2^28-1 or ldx above 2^34 is not supported", who);
   TYLO_REQUIRE(temperature > 0.f && temperature <= 3.0e38f && 1.f / temperature <= 1e30f, TYLO_ERR_INVALID_ARGUMENT,
                "%s: temperature must be positive and finite", who);
   TYLO_REQUIRE(aligned16(X), TYLO_ERR_MISALIGNED, "%s: X must be 16-byte aligned", who);
