@@ -1,5 +1,8 @@
 """GPU: log probabilities of tokens with entropy and alternatives, and distillation from a teacher's top logits, forward, backward and
 in one launch, against the oracle in 64 bits.  Tolerances are derived in vocab_util.py."""
+import threading
+from concurrent.futures import ThreadPoolExecutor
+
 import numpy as np
 import pytest
 import torch
@@ -389,6 +392,39 @@ def test_captured_replayed_and_on_another_stream(tylo):
         for k in want:
             for x, y in zip(want[k] if isinstance(want[k], tuple) else [want[k]], b[k] if isinstance(b[k], tuple) else [b[k]]):
                 assert torch.equal(x, y), k
+
+
+def test_calls_of_several_threads(tylo):
+    """Rows of different lengths that take the same kernel, whose needs of shared memory differ, from threads that run at once."""
+    lengths = (34000, 40000, 47000, 54000)
+    rng = np.random.default_rng(12)
+    data = []
+    for M in lengths:
+        X, _, _ = logits(rng, 600, M, "bf16")
+        t, g = dev(rng.integers(0, M, 600), torch.int32), torch.ones(600, device="cuda")
+        teacher, index = dev(rng.standard_normal((600, 4))), dev(rng.integers(0, M, (600, 4)), torch.int32)
+        data.append((X, t, g, teacher, index))
+
+    def both(X, t, g, teacher, index):
+        logp, loss, d1, d2 = torch.empty_like(g), torch.empty_like(g), torch.empty_like(X), torch.empty_like(X)
+        tylo.token_logprobs_with_grad_(tylo.Duplicated(logp, g), tylo.Duplicated(X, d1), t)
+        tylo.distill_with_grad_(tylo.Duplicated(loss, g), tylo.Duplicated(X, d2), teacher, index)
+        return logp, loss, d1, d2
+
+    want = [both(*d) for d in data]
+    torch.cuda.synchronize()
+    start = threading.Barrier(len(data))
+
+    def work(i):
+        start.wait(60)
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(100):
+                got = both(*data[i])
+            torch.cuda.current_stream().synchronize()
+            return all(torch.equal(a, b) for a, b in zip(got, want[i]))
+
+    with ThreadPoolExecutor(len(data)) as pool:
+        assert all(pool.map(work, range(len(data))))
 
 
 @pytest.mark.parametrize("N,M", [(1, 131072), (33, 50001), (400, 8192)])

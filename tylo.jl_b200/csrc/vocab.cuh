@@ -782,11 +782,18 @@ __device__ __forceinline__ uint32_t vocab_mine(const T* x, const VocabRow<T>& r,
   return k;
 }
 
+// Rows of up to this many packets per CTA wait in shared memory for their second look: 106 KB, two CTAs per SM.
+constexpr int kResident = 6784;
+// Most dynamic shared memory of a launch: such a row with its teacher's entries.  Where a kernel may need more than the default, the limit
+// is raised to this, not to what the call needs: calls of other sizes may be under way on other threads between the raise and the launch.
+constexpr int kVocabMaxShared = kResident * 16 + 12 * TYLO_DISTILL_MAX;
+static_assert(sizeof(TopScratch<512>) <= kVocabMaxShared, "alternatives");
+
 // Launches `parts` CTAs per row, as a cluster where they have something to tell one another.
 template <typename A>
 int32_t launch_vocab(const char* who, void (*kernel)(A, int), const A& args, int64_t N, int parts, int threads, cudaStream_t stream, int smem = 0) {
   if (smem > 40 * 1024)       // (with the kernels' own arrays; the default limit is 48 KB)
-    TYLO_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    TYLO_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kVocabMaxShared));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(N * parts));
   cfg.blockDim = dim3(threads);
@@ -798,7 +805,11 @@ int32_t launch_vocab(const char* who, void (*kernel)(A, int), const A& args, int
   cfg.attrs = attr;
   cfg.numAttrs = parts > 1 ? 1 : 0;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args, parts);
-  if (e != cudaSuccess) { set_error("launch of %s failed: %s", who, cudaGetErrorString(e)); return TYLO_ERR_CUDA; }
+  if (e != cudaSuccess) {
+    cudaGetLastError();                     // it is told here: the next launch's check is not to find it
+    set_error("launch of %s failed: %s", who, cudaGetErrorString(e));
+    return TYLO_ERR_CUDA;
+  }
   return TYLO_OK;
 }
 
@@ -824,7 +835,6 @@ inline int vocab_parts_twice(int64_t N, int64_t packets, int64_t pair) {
 
 // Shape of a kernel that looks at its row twice: rows of up to kResident packets per CTA wait in shared memory.  Value and gradient, bf16, us,
 // waiting / read again: 8192 x 16000 81 / 90, 4096 x 32768 83 / 93, 2048 x 50000 75 / 77.
-constexpr int kResident = 6784;           // 106 KB: two CTAs per SM
 #define TYLO_VOCAB_RESIDENT(LAUNCH)                                      \
   if (per <= 1024) return LAUNCH(128, 4, 2);                             \
   if (per <= 2048) return LAUNCH(128, 4, 4);                             \
