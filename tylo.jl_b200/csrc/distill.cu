@@ -7,7 +7,7 @@
 //
 // Entries with an index outside [0, M) are left out, of the teacher's normalisation too.
 //
-// Bound and shapes as in logprob.cu; the entries come on top: 64 of them cost the forward nothing that shows (4096 x 65536 bf16 87 us), 128
+// Bound and shapes as in logprob.cu; the entries come on top: 64 of them cost the forward little (4096 x 65536 bf16 87 us, 83 without), 128
 // cost value and gradient of 4096 x 32768 15 us of 107, of 4096 x 131072 25 of 425, and the backward of 4096 x 32768 12 of 97.  The entries
 // of a row are dealt with by one warp, so their sums are the same for every shape; an index that occurs more than once is summed in
 // the order of the entries by whoever stores it, so no order of the GPU's shows.
@@ -24,7 +24,7 @@ struct DistillArgs {
   const float* dLoss;
   const float *inMx, *inL;
   int64_t ldx;
-  int M, K, renormalize;
+  int M, K, renormalize, sms;
   float temperature, teacher_temperature;
 };
 
@@ -113,10 +113,12 @@ distill_row_kernel(const DistillArgs a, int parts) {
   const int slots = entry_slots(a.K);
   const Entries e(dynamic, slots);
   uint4* kept = reinterpret_cast<uint4*>(e.index + slots);
-  const size_t row = blockIdx.x / parts;
+  // (the gradient alone goes from the last row to the first: what the forward read last is still in L2)
+  const unsigned block = LOSS ? blockIdx.x : gridDim.x - 1 - blockIdx.x;
+  const size_t row = block / parts;
   const T* x = (const T*)a.X + row * a.ldx;
   const VocabRow<T> r(x, a.M);
-  const VocabPart part(blockIdx.x % parts, parts, r.whole);
+  const VocabPart part(block % parts, parts, r.whole);
   const float it = 1.f / a.temperature, scale = kVocabLog2e / a.temperature;
   const bool on_row = !EXTRA || threadIdx.x < THREADS;
   const bool on_entries = EXTRA ? threadIdx.x >= THREADS : threadIdx.x < 32;      // a warp
@@ -130,6 +132,7 @@ distill_row_kernel(const DistillArgs a, int parts) {
       st = vocab_resident_stats<T, THREADS, U, GROUPS, false>(kept, x, r, part, scale);
     } else if constexpr (LOSS) {
       st = vocab_thread_stats<T, THREADS, U, false, GRAD, false>(x, r, part, scale, nullptr);
+      if constexpr (!GRAD) vocab_ask_ahead((const T*)a.X, a.ldx, a.M, row, a.sms * distill_ctas(THREADS, GROUPS, GRAD), parts);
     } else {
       st = {a.inMx[row], 0.f, a.inL[row], 0.f};
     }
@@ -250,7 +253,7 @@ static int32_t check_distill(const char* who, const void* X, const float* teache
 static DistillArgs distill_args(const void* X, const float* teacher, const int32_t* index, int32_t K, int64_t M, int64_t ldx,
                                 float temperature, float teacher_temperature, int32_t renormalize) {
   DistillArgs a = {};
-  a.X = X; a.teacher = teacher; a.index = index; a.K = K; a.M = (int)M; a.ldx = ldx;
+  a.X = X; a.teacher = teacher; a.index = index; a.K = K; a.M = (int)M; a.ldx = ldx; a.sms = sm_count();
   a.temperature = temperature; a.teacher_temperature = teacher_temperature; a.renormalize = renormalize;
   return a;
 }

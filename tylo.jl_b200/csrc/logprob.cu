@@ -3,14 +3,14 @@
 //   logp = y_target - log L,   H = log L - A / L,   A = sum exp(y) y                      (y, L as in vocab.cuh)
 //   dX_j = 1/t ( g ([j = target] - p_j) - h p_j (log p_j + H) )
 //
-// Forward: one pass over the row, which memory bounds: 2048 x 131072 bf16 in 85 us = 6.3 TB/s (a plain read of the same bytes takes 76),
-// 4096 x 131072 in 159 us = 6.8 TB/s; the special-function units, one exponential per logit, are three quarters busy beside it.  Smaller
-// CTAs for shorter rows, so that starting a CTA and joining its sums weigh less: 4096 x 32768 50 us with 256 threads, 8192 x 16000 50 us
-// with 128 and 67 with 512.  With 20 alternatives 104 us for 2048 x 131072 and 69 for 4096 x 32768, with 128 of them 122 and 96: what
-// follows the sums is a chain of short steps (without it the same kernel takes 88 and 54), hidden by the other CTAs of the SM only.
+// Forward: one pass over the row, which memory bounds: 2048 x 131072 bf16 in 79 us = 6.8 TB/s (a plain read of the same bytes takes 76);
+// the special-function units, one exponential per logit, are three quarters busy beside it.  Smaller CTAs for shorter rows, so that
+// starting a CTA and joining its sums weigh less: 4096 x 32768 44 us with 256 threads, 8192 x 16000 45 us with 128 (67 with 512).  With
+// 20 alternatives 102 us for 2048 x 131072 and 64 for 4096 x 32768, with 128 of them 121 and 93: what follows the sums is a chain of
+// short steps (without it the same kernel takes 88 and 54), hidden by the other CTAs of the SM only.
 // Backward: one read and one write, 4096 x 65536 bf16 159 us = 6.8 TB/s, with the entropy's weight 161 us.
 // Value and gradient in one launch read the logits from memory once: 4096 x 32768 bf16 91 us = 5.9 TB/s (98 us under the power cap of a
-// longer run) against 135 for the two calls, 2048 x 131072 196 us (the second look finds two thirds of a longer row in L2).
+// longer run) against 128 for the two calls, 2048 x 131072 196 us (the second look finds two thirds of a longer row in L2).
 #include "vocab.cuh"
 
 namespace tylo {
@@ -24,7 +24,7 @@ struct LogprobArgs {
   const float *dLogp, *dEntropy;
   const float *inEntropy, *inMx, *inL;
   int64_t ldx;
-  int M, top;
+  int M, top, sms;
   float temperature;
 };
 
@@ -92,6 +92,7 @@ __global__ void __launch_bounds__(THREADS, logprob_ctas(THREADS, ENTROPY, TOP)) 
   VocabStats st = vocab_thread_stats<T, THREADS, 4, ENTROPY, false, TOP>(x, r, part, scale, &cells);
   const bool has = target >= 0 && target < a.M;
   const float xt = has ? Elem<T>::to_f(x[target]) : 0.f;
+  vocab_ask_ahead((const T*)a.X, a.ldx, a.M, row, a.sms * logprob_ctas(THREADS, ENTROPY, TOP), parts);
   const bool odd = st.s != st.s;
   if constexpr (TOP) top.mine[threadIdx.x] = vocab_mine<T, THREADS>(x, r, part, st);
   vocab_reduce<THREADS, ENTROPY>(st, scale, scratch, parts);
@@ -145,13 +146,14 @@ logprob_fwd_bwd_kernel(const LogprobArgs a, int parts) {
 }
 
 // 2,048 packets per CTA: a row's coefficients cost a thread as much as three packets (1,024: 4096 x 65536 bf16 with both weights 200 us,
-// 161 with 2,048).
+// 161 with 2,048).  From the last row to the first: what the forward read last is still in L2 (forward and backward, 4096 x 32768 bf16 133
+// and 128.5 us, 777 x 50001 fp32 83.3 and 81.6, 4096 x 65536 259.9 and 256.4).
 template <typename T, int THREADS, bool ENTROPY>
 __global__ void __launch_bounds__(THREADS, 6) logprob_bwd_kernel(const LogprobArgs a, int parts) {
-  const size_t row = blockIdx.x / parts;
+  const size_t row = (gridDim.x - 1 - blockIdx.x) / parts;
   const T* x = (const T*)a.X + row * a.ldx;
   const VocabRow<T> r(x, a.M);
-  const VocabPart part(blockIdx.x % parts, parts, r.whole);
+  const VocabPart part((gridDim.x - 1 - blockIdx.x) % parts, parts, r.whole);
   const int target = a.targets ? a.targets[row] : -1;
   const bool has = target >= 0 && target < a.M;
   const float xt = has ? Elem<T>::to_f(x[target]) : 0.f;
@@ -218,7 +220,7 @@ extern "C" int32_t tylo_b200_token_logprobs_fwd(float* Logp, float* Entropy, flo
                "%s: TopLogp and TopIndex go with top > 0", who);
   LogprobArgs a = {};
   a.X = X; a.targets = targets; a.Logp = Logp; a.Entropy = Entropy; a.TopLogp = TopLogp; a.TopIndex = TopIndex; a.Mx = Mx; a.L = L;
-  a.ldx = ldx; a.M = (int)M; a.top = top; a.temperature = temperature;
+  a.ldx = ldx; a.M = (int)M; a.top = top; a.sms = sm_count(); a.temperature = temperature;
   TYLO_DISPATCH_DTYPE(dtype, T, return (Entropy ? logprob_fwd_dispatch<T, true>(who, a, N, (cudaStream_t)stream)
                                                 : logprob_fwd_dispatch<T, false>(who, a, N, (cudaStream_t)stream)));
   return TYLO_OK;
