@@ -7,7 +7,7 @@
 //
 // Entries with an index outside [0, M) are left out, of the teacher's normalisation too.
 //
-// Bound and shapes as in logprob.cu; the entries come on top: 64 of them cost the forward little (4096 x 65536 bf16 87 us, 83 without), 128
+// Bound and shapes as in logprob.cu; the entries come on top: 64 of them cost the forward nothing that shows (4096 x 65536 bf16 87 us), 128
 // cost value and gradient of 4096 x 32768 15 us of 107, of 4096 x 131072 25 of 425, and the backward of 4096 x 32768 12 of 97.  The entries
 // of a row are dealt with by one warp, so their sums are the same for every shape; an index that occurs more than once is summed in
 // the order of the entries by whoever stores it, so no order of the GPU's shows.
@@ -71,9 +71,11 @@ __device__ __forceinline__ void load_entries(const DistillArgs& a, const Entries
 }
 
 // By one warp, all lanes: probabilities exp((v_k - m) / u) / S from values v_k (the difference first: the lowest value overflows where it
-// is divided by less than 1); returns their sum, and m and log S.
+// is divided by less than 1; a factor 1 / u, for a quotient of each entry costs 10 us of 50 for 4096 x 32768 bf16 with 128);
+// returns their sum, and m and log S.
 __device__ __forceinline__ float teacher_probabilities(const DistillArgs& a, const Entries& e, float& m, float& log_sum) {
   const int lane = threadIdx.x & 31;
+  const float iu = 1.f / a.teacher_temperature;
   m = log_sum = 0.f;
   if (a.renormalize) {
     float most = -INFINITY;
@@ -83,7 +85,7 @@ __device__ __forceinline__ float teacher_probabilities(const DistillArgs& a, con
   }
   float sum = 0.f;
   for (int k = lane; k < a.K; k += 32) {
-    const float p = expf((e.p[k] - m) / a.teacher_temperature);
+    const float p = expf((e.p[k] - m) * iu);
     e.p[k] = p;
     sum += p;
   }
@@ -119,12 +121,12 @@ distill_row_kernel(const DistillArgs a, int parts) {
   const T* x = (const T*)a.X + row * a.ldx;
   const VocabRow<T> r(x, a.M);
   const VocabPart part(block % parts, parts, r.whole);
-  const float it = 1.f / a.temperature, scale = kVocabLog2e / a.temperature;
+  const float scale = kVocabLog2e / a.temperature;
   const bool on_row = !EXTRA || threadIdx.x < THREADS;
   const bool on_entries = EXTRA ? threadIdx.x >= THREADS : threadIdx.x < 32;      // a warp
   const int lane = threadIdx.x & 31;
   float w = 0.f, teacher_max = 0.f, teacher_log = 0.f;
-  if constexpr (GRAD) w = a.dLoss[row] * it;
+  if constexpr (GRAD) w = a.dLoss[row] / a.temperature;
   VocabStats st{-INFINITY, -INFINITY, 0.f, 0.f};
   if (on_row) {
     if constexpr (GROUPS > 0) {
@@ -132,7 +134,6 @@ distill_row_kernel(const DistillArgs a, int parts) {
       st = vocab_resident_stats<T, THREADS, U, GROUPS, false>(kept, x, r, part, scale);
     } else if constexpr (LOSS) {
       st = vocab_thread_stats<T, THREADS, U, false, GRAD, false>(x, r, part, scale, nullptr);
-      if constexpr (!GRAD) vocab_ask_ahead((const T*)a.X, a.ldx, a.M, row, a.sms * distill_ctas(THREADS, GROUPS, GRAD), parts);
     } else {
       st = {a.inMx[row], 0.f, a.inL[row], 0.f};
     }
@@ -150,6 +151,8 @@ distill_row_kernel(const DistillArgs a, int parts) {
     vocab_reduce<THREADS, false>(st, scale, scratch, parts);      // its barriers publish the entries
   } else {
     load_entries<T, THREADS>(a, e, row, x, threadIdx.x, slots);
+    // (long rows only: 2048 x 131072 bf16 with 64 entries 87 us without and 83 so, but 4096 x 65536 87 and 94, 8192 x 16000 52 and 57)
+    if constexpr (LOSS && THREADS == 512) vocab_ask_ahead((const T*)a.X, a.ldx, a.M, row, a.sms * distill_ctas(THREADS, GROUPS, GRAD), parts);
     if constexpr (LOSS) vocab_reduce<THREADS, false>(st, scale, scratch, parts);
     else __syncthreads();
     if (on_entries && (GRAD || part.part == 0)) probabilities();
@@ -159,10 +162,11 @@ distill_row_kernel(const DistillArgs a, int parts) {
   if (LOSS && on_entries && part.part == 0) {
     const float logL = st.s == 0.f ? 0.f : logf(st.s);
     const float* teacher = a.teacher + row * a.K;
+    const float it = 1.f / a.temperature, iu = 1.f / a.teacher_temperature;     // (here: no registers for them in the loops above)
     float loss = 0.f;
     for (int k = lane; k < a.K; k += 32) {
       const float p = e.p[k];
-      if (e.index[k] >= 0 && p != 0.f) loss += p * (((teacher[k] - teacher_max) / a.teacher_temperature - teacher_log) - ((e.xk[k] - mo) / a.temperature - logL));
+      if (e.index[k] >= 0 && p != 0.f) loss += p * (((teacher[k] - teacher_max) * iu - teacher_log) - ((e.xk[k] - mo) * it - logL));
     }
     loss = warp_reduce(loss, SumOp());
     if (lane == 0) {
