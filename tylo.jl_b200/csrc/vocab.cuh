@@ -530,10 +530,12 @@ __device__ __noinline__ int vocab_top(const T* x, const VocabRow<T> r, const Voc
         }
       }
     } else {
-      lo = 1;                               // below every element
+      // fewer threads hold data than K: the key of the smallest value.  The bound, and every bound raised from it, has to be a number's
+      // key or lie above all numbers': a NaN's below it would compare as false with every cell.
+      lo = vocab_key(-INFINITY);
     }
     // (many maxima equal to the bound, as where a mask leaves little: its equals would not fit, so they are not tried)
-    if (lane == 0) { sc.bound = lo; sc.most = most; sc.dense = lo > 1 && reach >= 2 * K + 32; sc.n = 0; sc.m = 0; }
+    if (lane == 0) { sc.bound = lo; sc.most = most; sc.dense = reach >= 2 * K + 32; sc.n = 0; sc.m = 0; }
   }
   __syncthreads();
   uint32_t t = sc.bound, lo, hi;
@@ -553,7 +555,7 @@ __device__ __noinline__ int vocab_top(const T* x, const VocabRow<T> r, const Voc
     }
     const bool any = mine >= from;
     if (!__any_sync(0xffffffffu, any)) return;
-    const float low = from <= 1 ? -INFINITY : vocab_unkey(from);       // (without a value of its own it is a NaN: `all` alone counts)
+    const float low = vocab_unkey(from);       // (above the key of +Inf it is a NaN: `all` alone counts)
     uint16_t* hits = sc.hits[warp];
     static_assert(U == 4, "packets of a cell as a power of two");
     const int lg = cells.shift + 2, per = 1 << lg;
@@ -585,7 +587,7 @@ __device__ __noinline__ int vocab_top(const T* x, const VocabRow<T> r, const Voc
   };
   // elements above or at a bound into sc.keys; more than kTopSlots: at least that many
   auto collect = [&](uint32_t from) {
-    const float low = from <= 1 ? -INFINITY : vocab_unkey(from);
+    const float low = vocab_unkey(from);
     visit(from, [&](const Pack<T>& p, uint32_t there, int first) {
       float e[VEC];
       p.unpack(e);
@@ -640,7 +642,7 @@ __device__ __noinline__ int vocab_top(const T* x, const VocabRow<T> r, const Voc
       n = collect(t);
       if (n > kTopSlots) { clear(); n = above(t); }
     }
-    if (n < K) {
+    if (n < K) {       // (at least K elements reach t, whichever way it was found)
       // the elements equal to the bound, lowest index first: they are counted off in blocks of THREADS packets
       const int need = K - n;
       int taken = 0;
