@@ -1,0 +1,26 @@
+"""CPU: the ChainRules rules of the vocabulary operators, read as text (the Julia sources cannot be executed here)."""
+import re
+from pathlib import Path
+
+TYLO = Path(__file__).resolve().parent.parent / "tylo.jl_b200" / "julia" / "Tylo"
+RULES = (TYLO / "ext" / "ChainRulesCoreExt.jl").read_text()
+
+
+def body(text, opening):
+    """A top-level function, from `opening` to the `end` in the first column."""
+    at = text.index(opening)
+    return text[at:text.index("\nend", at)]
+
+
+def rule(name):
+    return re.sub(r"#.*", "", body(RULES, f"function rrule(::typeof({name})"))
+
+
+def test_every_result_of_the_scores_has_its_cotangent_looked_at():
+    """A field of the result whose cotangent the pullback never reads would drop a gradient without a word."""
+    primal = body((TYLO / "src" / "vocab" / "logprobs.jl").read_text(), "function token_logprobs(")
+    fields = [f.split("=")[0].strip() for f in re.search(r"return \(;\s*(.*)\)", primal).group(1).split(",")]
+    assert fields == ["logp", "entropy", "top"]
+    for f in fields:
+        assert f"Ȳ.{f}" in rule("token_logprobs"), f
+    assert "throw(ArgumentError(" in rule("token_logprobs")        # the alternatives' cotangent, which has no kernel

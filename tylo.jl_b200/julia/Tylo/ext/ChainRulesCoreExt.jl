@@ -45,12 +45,17 @@ function rrule(::typeof(softmax), X)
     return Y, pullback
 end
 
-# the alternatives are a report: no gradient runs through them; the cotangent of a value that is not used is a zero tangent
+# the cotangent of a value that is not used is a zero tangent; the alternatives are a report, through which no gradient runs: a
+# cotangent of their log probabilities is refused, not dropped
 function rrule(::typeof(token_logprobs), X, targets; temperature = 1, entropy = false, top = 0)
     cp = allocate_checkpoints(token_logprobs!, X)
     out = token_logprobs(X, targets; temperature, entropy, top, checkpoints = cp)
     function pullback(Ȳ)
         Ȳ = unthunk(Ȳ)
+        Ȳ isa AbstractZero && return NoTangent(), NoTangent(), NoTangent()
+        t̄ = unthunk(Ȳ.top)
+        t̄ isa AbstractZero || unthunk(t̄.logp) isa AbstractZero ||
+            throw(ArgumentError("token_logprobs: no gradient runs through the alternatives; use them under ignore_derivatives"))
         l̄ = targets === nothing ? NoTangent() : unthunk(Ȳ.logp)
         ē = entropy ? unthunk(Ȳ.entropy) : NoTangent()
         l̄ isa AbstractZero && ē isa AbstractZero && return NoTangent(), NoTangent(), NoTangent()

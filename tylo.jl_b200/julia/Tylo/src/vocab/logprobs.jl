@@ -36,7 +36,8 @@ allocate_top(X, K) = (; logp = similar(X, Float32, K, size(X, 2)), index = simil
     token_logprobs!(logp, X, targets; temperature = 1, entropy = nothing, top = nothing, checkpoints = nothing) -> logp
 
 Log probabilities of `targets (N,)` under `softmax(X / temperature)` per column of `X (M,N)`, and, where a buffer is given, the
-`entropy (N,)` and the largest alternatives `top = allocate_top(X, K)`.  `logp` and `targets` may both be `nothing`.
+`entropy (N,)` and the largest alternatives `top = allocate_top(X, K)`.  `logp` and `targets` may both be `nothing`.  The alternatives
+are a report: no gradient runs through them, and the rule of `token_logprobs` refuses a cotangent of theirs.
 """
 function token_logprobs!(logp, X, targets; temperature = 1, entropy = nothing, top = nothing, checkpoints = nothing)
     px, pl, pe = primal(X), primal(logp), primal(entropy)
