@@ -24,3 +24,22 @@ def test_every_result_of_the_scores_has_its_cotangent_looked_at():
     for f in fields:
         assert f"Ȳ.{f}" in rule("token_logprobs"), f
     assert "throw(ArgumentError(" in rule("token_logprobs")        # the alternatives' cotangent, which has no kernel
+
+
+def keywords(signature):
+    """Names of the keyword arguments of a one-line function signature; splats keep their dots."""
+    inside = signature[signature.index(";") + 1:signature.rindex(")")]
+    return {k.split("=")[0].strip() for k in inside.split(",")}
+
+
+def test_the_rule_takes_the_keywords_of_the_operator():
+    source = (TYLO / "src" / "vocab" / "logprobs.jl").read_text()
+    assert keywords(rule("token_logprobs").split("\n")[0]) == keywords(body(source, "function token_logprobs(").split("\n")[0])
+
+
+def test_checkpoints_given_by_the_caller_reach_forward_and_backward():
+    for name in ("token_logprobs", "distill"):
+        text = rule(name)
+        assert "checkpoints = nothing" in text.split("\n")[0], name
+        assert "cp = checkpoints === nothing ?" in text, name
+        assert text.count("checkpoints = cp") == 2, name

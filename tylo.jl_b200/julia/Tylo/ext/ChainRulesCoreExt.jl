@@ -47,8 +47,8 @@ end
 
 # the cotangent of a value that is not used is a zero tangent; the alternatives are a report, through which no gradient runs: a
 # cotangent of their log probabilities is refused, not dropped
-function rrule(::typeof(token_logprobs), X, targets; temperature = 1, entropy = false, top = 0)
-    cp = allocate_checkpoints(token_logprobs!, X)
+function rrule(::typeof(token_logprobs), X, targets; temperature = 1, entropy = false, top = 0, checkpoints = nothing)
+    cp = checkpoints === nothing ? allocate_checkpoints(token_logprobs!, X) : checkpoints
     out = token_logprobs(X, targets; temperature, entropy, top, checkpoints = cp)
     function pullback(Ȳ)
         Ȳ = unthunk(Ȳ)
@@ -67,8 +67,8 @@ function rrule(::typeof(token_logprobs), X, targets; temperature = 1, entropy = 
     return out, pullback
 end
 
-function rrule(::typeof(distill), X, teacher, index; kwargs...)
-    cp = allocate_checkpoints(distill!, X)
+function rrule(::typeof(distill), X, teacher, index; checkpoints = nothing, kwargs...)
+    cp = checkpoints === nothing ? allocate_checkpoints(distill!, X) : checkpoints
     loss = distill(X, teacher, index; checkpoints = cp, kwargs...)
     pullback(loss̄) = (NoTangent(), ∇distill(unthunk(loss̄), X, teacher, index; checkpoints = cp, kwargs...), NoTangent(), NoTangent())
     return loss, pullback
