@@ -43,3 +43,10 @@ def test_checkpoints_given_by_the_caller_reach_forward_and_backward():
         assert "checkpoints = nothing" in text.split("\n")[0], name
         assert "cp = checkpoints === nothing ?" in text, name
         assert text.count("checkpoints = cp") == 2, name
+
+
+def test_a_loss_that_is_not_used_has_a_zero_gradient():
+    """The pullback may be handed a zero tangent, which has no memory to give to a kernel."""
+    for name in ("token_logprobs", "distill"):
+        pullback = rule(name)[rule(name).index("pullback("):]
+        assert "isa AbstractZero" in pullback[:pullback.index("∇" + name)], name

@@ -67,10 +67,15 @@ function rrule(::typeof(token_logprobs), X, targets; temperature = 1, entropy = 
     return out, pullback
 end
 
+# the teacher's entries are constants of the operator, also where they come from a differentiated call
 function rrule(::typeof(distill), X, teacher, index; checkpoints = nothing, kwargs...)
     cp = checkpoints === nothing ? allocate_checkpoints(distill!, X) : checkpoints
     loss = distill(X, teacher, index; checkpoints = cp, kwargs...)
-    pullback(loss̄) = (NoTangent(), ∇distill(unthunk(loss̄), X, teacher, index; checkpoints = cp, kwargs...), NoTangent(), NoTangent())
+    function pullback(l̄)
+        l̄ = unthunk(l̄)
+        l̄ isa AbstractZero && return NoTangent(), NoTangent(), NoTangent(), NoTangent()
+        return NoTangent(), ∇distill(l̄, X, teacher, index; checkpoints = cp, kwargs...), NoTangent(), NoTangent()
+    end
     return loss, pullback
 end
 

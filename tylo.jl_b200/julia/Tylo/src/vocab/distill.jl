@@ -15,6 +15,7 @@ end
 `loss (N,) = Σₖ Pₖ (log Pₖ − log softmax(X / temperature)[indexₖ])`.  With `renormalize`, `P` is the softmax of
 `teacher / teacher_temperature` over the row's entries, otherwise its exponential as it is.  The alternatives of `token_logprobs!`
 already have their temperature in them: they go with `teacher_temperature = 1`.  Entries with an id outside `0:M-1` are left out.
+The teacher's entries are constants: no gradient runs into them.
 """
 function distill!(loss, X, teacher, index; temperature = 1, teacher_temperature = temperature, renormalize = true, checkpoints = nothing)
     px, pl = primal(X), primal(loss)
