@@ -7,8 +7,10 @@
 //
 // Entries with an index outside [0, M) are left out, of the teacher's normalisation too.
 //
-// Bound and shapes as in logprob.cu; the entries come on top: 64 of them cost the forward nothing that shows (4096 x 65536 bf16 87 us), 128
-// cost value and gradient of 4096 x 32768 15 us of 107, of 4096 x 131072 25 of 425, and the backward of 4096 x 32768 12 of 97.  The entries
+// Bound, shapes and how times are taken as in logprob.cu; the entries come on top.  us, bf16: the loss with 64 entries 2048 x 131072 96, 4096 x
+// 65536 96, 512 x 131072 29; of 4096 x 32768 with 1 52, with 128 58.  Value and gradient of 4096 x 32768 with 1 / 128 / 256 / 512 / 1,024
+// entries 103 / 120 / 147 / 270 / 936, of 4096 x 131072 with 1 / 128 / 1,024 431 / 445 / 915: every entry is compared with every other for
+// copies of its index.  The backward with 1 and 128 entries: 4096 x 32768 91 and 107, 4096 x 65536 171 and 195.  The entries
 // of a row are dealt with by one warp, so their sums are the same for every shape; an index that occurs more than once is summed in
 // the order of the entries by whoever stores it, so no order of the GPU's shows.
 #include "vocab.cuh"

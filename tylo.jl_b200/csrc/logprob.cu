@@ -3,14 +3,24 @@
 //   logp = y_target - log L,   H = log L - A / L,   A = sum exp(y) y                      (y, L as in vocab.cuh)
 //   dX_j = 1/t ( g ([j = target] - p_j) - h p_j (log p_j + H) )
 //
-// Forward: one pass over the row, which memory bounds: 2048 x 131072 bf16 in 79 us = 6.8 TB/s (a plain read of the same bytes takes 76);
-// the special-function units, one exponential per logit, are three quarters busy beside it.  Smaller CTAs for shorter rows, so that
-// starting a CTA and joining its sums weigh less: 4096 x 32768 44 us with 256 threads, 8192 x 16000 45 us with 128 (67 with 512).  With
-// 20 alternatives 102 us for 2048 x 131072 and 64 for 4096 x 32768, with 128 of them 121 and 93: what follows the sums is a chain of
-// short steps (without it the same kernel takes 88 and 54), hidden by the other CTAs of the SM only.
-// Backward: one read and one write, 4096 x 65536 bf16 159 us = 6.8 TB/s, with the entropy's weight 161 us.
-// Value and gradient in one launch read the logits from memory once: 4096 x 32768 bf16 91 us = 5.9 TB/s (98 us under the power cap of a
-// longer run) against 128 for the two calls, 2048 x 131072 196 us (the second look finds two thirds of a longer row in L2).
+// Times are us of a pass among others in runs of a second and more, where the card is at its power cap; short runs take up to a tenth less,
+// cards differ by a twentieth.  bf16 unless said otherwise.
+// Forward: one pass over the row, which memory bounds: 2048 x 131072 86 to 90 = 6.2 TB/s (a plain read of the same bytes takes 76 in short
+// runs, this 79), fp16 91, 1024 x 131072 fp32 80; with the entropy 4096 x 65536 99.  The special-function units, one exponential per logit,
+// are three quarters busy beside it.  Smaller CTAs for shorter rows, so that starting a CTA and joining its sums weigh less: 4096 x 32768 46
+// to 49 with 256 threads, 8192 x 16000 50 with 128 (67 with 512 when that was chosen).  Below that the CTA a row costs more than the row:
+// 8192 x 4000 19 for 10 us of bytes, 8192 x 1000 16 for 2.5.
+// Alternatives: what follows the sums is a chain of short steps, hidden by the other CTAs of the SM only.
+//   alternatives      0    20   128   256                            0    20    64   128   256
+//   2048 x 131072    86   103   122   157      8192 x 4000           19    50    64   117   293
+//   4096 x 32768     46    65    94   168      8192 x 1000           16    47    64   211   365
+//   8192 x 16000     49    78   139   287      8192 x 1100, 150: 511 (the bound is below every element, and raised)
+// A mask that leaves 40: 256 x 32000 fp16 with 64 of them 13.2 and 16.4 masked, with 200 16.4 and 20.6; 3000 x 1000 with 100 58 and 165, with
+// 256 141 and 262.
+// Backward: one read and one write, 4096 x 65536 160 = 6.7 TB/s, with the entropy's weight 171.
+// Value and gradient in one launch read the logits from memory once: 4096 x 32768 104 to 107 = 5.1 TB/s, with the entropy 113, fp16 105, 2048 x
+// 32768 fp32 96, the two calls with the entropy 139; 8192 x 16000 103.  The second look finds two thirds of a longer row in L2: 2048 x 131072
+// 210, 1024 x 131072 fp32 217, 2048 x 262144 431.  Rows whose target is no token are read all the same: half of them such, 99 and 195.
 #include "vocab.cuh"
 
 namespace tylo {
@@ -111,8 +121,8 @@ __global__ void __launch_bounds__(THREADS, logprob_ctas(THREADS, ENTROPY, TOP)) 
   cluster_done(parts);
 }
 
-// Value and gradient.  GROUPS > 0: the part waits in shared memory for the second look (4096 x 32768 bf16 91 us; read again from L2 it
-// took 105); 0: it is too long for that and is read again, out of L2 as far as it is still there.
+// Value and gradient.  GROUPS > 0: the part waits in shared memory for the second look; 0: it is too long for that and is read again, out of
+// L2 as far as it is still there (both sides: TYLO_VOCAB_RESIDENT).
 template <typename T, int THREADS, int U, int GROUPS, bool ENTROPY>
 __global__ void __launch_bounds__(THREADS, THREADS == 128 ? 8 : THREADS == 256 ? 5 : GROUPS ? 2 : 3)
 logprob_fwd_bwd_kernel(const LogprobArgs a, int parts) {
@@ -170,7 +180,7 @@ static int32_t logprob_fwd_dispatch(const char* who, const LogprobArgs& a, int64
   // us, bf16.  256 threads up to 176 alternatives (256 / 512 threads: 4096 x 32768 with 144 of them 105 / 132, with 200 136 / 143; 2048 x
   // 131072 129 / 133 and 147 / 142): with more, the threads' maxima bound too little.  128 for a clustered row, whose lists have to fit
   // into 4 * THREADS places.  128 threads for many short rows (256 / 128: 8192 x 16000 with 20 108 / 81, 4096 x 32768 78 / 71, 2048 x 131072
-  // with 64 115 / 123, 256 x 32000 13.2 / 15.6).
+  // with 64 115 / 123, 256 x 32000 13.2 / 15.6).  The rule was found on rows of 16,000 logits and more.
 #define TYLO_TOP(THREADS) \
   launch_vocab(who, logprob_fwd_kernel<T, THREADS, ENTROPY, true>, a, N, parts, THREADS, stream, (int)sizeof(TopScratch<THREADS>))
   if (a.top && a.top <= 64 && per <= 4096 && N * parts >= 8 * sm_count()) return TYLO_TOP(128);

@@ -7,6 +7,9 @@
 // Exponents are in units of log 2; the smallest that is used as a factor is kExpFloor, whose exp2 is zero: an entry of -Inf
 // adds 0 * kExpFloor = 0 where 0 * -Inf would be NaN.  The sum itself takes the exponent as it is, so a NaN or +Inf reaches it.
 // A row made only of -Inf has L = 0 and no probability anywhere.
+//
+// What the kernels take now stands at the heads of logprob.cu and distill.cu.  The figures in the comments below, and beside single choices
+// there, set two forms against each other at the time of the choice, in short runs: they hold as pairs.
 #pragma once
 #include <cooperative_groups.h>
 
@@ -52,7 +55,8 @@ __device__ __forceinline__ uint4 ld_logits(const void* p) {
 }
 
 // The same with a place in L2: a row that will be read again stays there before what is read or written once (4096 x 131072 bf16, value
-// and gradient 414 us, 454 without), and is the first to go when it has been.
+// and gradient 414 us, 454 without), and is the first to go when it has been.  (A row that gets zeros is not read again: it stays until
+// other rows push it out.)
 __device__ __forceinline__ uint64_t keep_policy() {
   uint64_t p;
   asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(p));
@@ -73,7 +77,7 @@ __device__ __forceinline__ uint4 ld_logits(const void* p, uint64_t policy) {
 // Running statistics of a row or of a part of it: largest logit, the reference that the exponentials are taken against, sum of
 // e = exp2((x - ref) * scale), sum of e times its exponent.  The reference follows the maximum only when that is more than
 // kRefSlack (in units of log 2) above it: sums in floating point are as good (the entropy's second sum to kRefSlack * 2^-24), and the
-// branch that rescales them stays rare (2048 x 131072 bf16 92 and 89 us).
+// branch that rescales them stays rare (2048 x 131072 bf16 92 us with the maximum as reference, 89 so).
 constexpr float kRefSlack = 8.f;
 
 struct VocabStats {
@@ -358,9 +362,9 @@ __device__ __forceinline__ VocabStats vocab_resident_stats(const uint4* row, con
   return sum.stats();
 }
 
-// Special-function units: a fourth of the exponentials as polynomials on the multiply-add pipes was slower everywhere (entropy 169 and
-// 181 us, value and gradient 91 and 93), and so was one fused multiply-add per exponent against a rounded reference (no change): what is
-// left is memory and, in longer runs, the power cap (1000 W, 1.76 GHz).
+// Special-function units: a fourth of the exponentials as polynomials on the multiply-add pipes was slower everywhere (bf16, ex2 alone and
+// so: entropy of 4096 x 131072 169 and 181 us, value and gradient of 4096 x 32768 91 and 93), and one fused multiply-add per exponent
+// against a rounded reference changed nothing: what is left is memory and, in longer runs, the power cap (1000 W, 1.76 GHz).
 
 // Gradient of a part that waits in shared memory (vocab_resident_stats): f(pair of logits) -> pair of gradients for every element,
 // rounded once, on the way out.
@@ -457,6 +461,8 @@ __device__ __forceinline__ int vocab_key_index(uint64_t k) { return 0x7fffffff -
 // to shared memory: little more than K elements unless many sit together in few shares or are equal.  Where they do not fit, the bound
 // is raised by counting, and equal elements at the bound are taken in the order of their index.  What is left is thinned by bisection
 // to K and a few, whose rank is counted.
+// It is made for rows whose threads hold many more packets than K: where K is a large part of the elements the bound discards little, and the
+// thinning, some thirty steps with up to four barriers each, is most of the time (figures in logprob.cu).
 constexpr int kRanked = TYLO_TOP_MAX + 32;       // most elements that are ranked: lists of 32, one more than can be asked for
 
 template <int THREADS> struct TopScratch {
@@ -534,7 +540,9 @@ __device__ __noinline__ int vocab_top(const T* x, const VocabRow<T> r, const Voc
       // key or lie above all numbers': a NaN's below it would compare as false with every cell.
       lo = vocab_key(-INFINITY);
     }
-    // (many maxima equal to the bound, as where a mask leaves little: its equals would not fit, so they are not tried)
+    // Many maxima equal to the bound, as where a mask leaves little: its equals would not fit, so they are not tried.  That many threads
+    // must hold data: it can be seen so for K up to 48, 112 and 240 with 128, 256 and 512 of them; for more the equals are collected until
+    // the places are full, and counted off then.
     if (lane == 0) { sc.bound = lo; sc.most = most; sc.dense = reach >= 2 * K + 32; sc.n = 0; sc.m = 0; }
   }
   __syncthreads();
@@ -798,7 +806,8 @@ __device__ __forceinline__ uint32_t vocab_mine(const T* x, const VocabRow<T>& r,
   return k;
 }
 
-// Rows of up to this many packets per CTA wait in shared memory for their second look: 106 KB, two CTAs per SM.
+// Rows of up to this many packets per CTA wait in shared memory for their second look: 106 KB, two CTAs per SM (one, where more than
+// about 560 entries of a teacher lie before a row of that length).
 constexpr int kResident = 6784;
 // Most dynamic shared memory of a launch: such a row with its teacher's entries.  Where a kernel may need more than the default, the limit
 // is raised to this, not to what the call needs: calls of other sizes may be under way on other threads between the raise and the launch.
@@ -829,7 +838,9 @@ int32_t launch_vocab(const char* who, void (*kernel)(A, int), const A& args, int
   return TYLO_OK;
 }
 
-// CTAs per row: a row is dealt over a cluster while rows alone leave SMs without a CTA.
+// CTAs per row: a row is dealt over a cluster while rows alone leave SMs without a CTA.  Forward, bf16, us with 1 / 2 / 4 CTAs per row: 148 x
+// 131072 14.2 / 15.5 / 15.2, with 20 alternatives 27.0 / 23.2 / 22.2; 300 x 131072 21.8 / 21.3 / 19.7, with 20 alternatives 29.3 / 27.9 /
+// 33.6; 600 x 65536 21.4 / 23.8 / 25.7; 512 x 262144 49.7 / 51.7 / 52.1.
 inline int vocab_parts(int64_t N, int64_t packets) {
   int parts = 1;
   while (parts < 8 && N * parts * 2 <= 2 * sm_count() && packets >= parts * 1024LL) parts *= 2;
